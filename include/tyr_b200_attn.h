@@ -227,6 +227,87 @@ int tyr_b200_attn_decode(const TyrAttnDecodeArgs* args, void* stream);
 #define TYR_ATTN_DECODE_STATIC_SCRATCH_BYTES (16u << 20)
 int tyr_b200_attn_decode_static(const TyrAttnDecodeArgs* args, void* stream);
 
+/* ------------------------------------------------------------------------
+ * A KV cache in pages: the rows of a sequence lie in pages of `page_size` rows that its row of the page table names,
+ * row r in row r % page_size of page table[r / page_size].  No counterpart in the reference, whose cache is one dense
+ * block of maxLen rows per sequence (Tyr/Model/Qwen/Attention.lean:54-68).  K and V pools are
+ * [n_pages, n_kv_head, page_size, head_dim] bf16 in any order of those axes with unit stride on the last one.
+ * Only entries that hold a row the call touches are read: those behind a sequence's last row, and those of pages that
+ * lie wholly between the first tokens and the window, may be anything (pages out of sight can be given back).
+ * An entry outside [0, n_pages) that would be used sets TYR_ATTN_STATUS_OUT_OF_RANGE and is not followed.
+ * ---------------------------------------------------------------------- */
+typedef struct TyrAttnPageTable {
+  const int32_t* table; /* DEVICE int32 [batch, max_pages] */
+  int64_t table_stride; /* elements between the rows of two sequences */
+  int32_t max_pages;    /* entries of a row; > 0 */
+  int32_t n_pages;      /* pages of the pool; > 0 */
+  int32_t page_size;    /* rows of a page; any number > 0, max_pages * page_size < 2^31 */
+} TyrAttnPageTable;
+
+/* Decode over a paged cache: one query token per sequence, as tyr_b200_attn_decode, the query at the position of the
+ * sequence's last key.  With window_size > 0 it sees the last window_size keys and the first n_sink
+ * ones (0: every key); what it does not see is not read.
+ * kv_lens must be in [0, max_kv_seq]: a sequence of length 0 (an idle slot) gets a zero row and LSE = -inf; a
+ * length outside is clamped and sets TYR_ATTN_STATUS_OUT_OF_RANGE.  A bad page table entry gives NaN rows.
+ * `weights`, when not NULL, is a running sum per (sequence, KV head, key): the call adds, for every visible key, the
+ * softmax weights that the query heads of the group gave it; entries of other keys stay as they are.  No atomics: the
+ * same bits each time.
+ * At most two launches, three with `weights`. */
+typedef struct TyrAttnPagedDecodeArgs {
+  const void* q; /* [batch, n_head, head_dim] */
+  void* o;       /* [batch, n_head, head_dim] */
+  float* lse;    /* [batch, n_head] or NULL */
+  const void* k; /* pools, 16-byte aligned */
+  const void* v;
+  TyrAttnPageTable pages;
+  const int32_t* kv_lens; /* DEVICE int32 [batch] */
+  float* weights;         /* DEVICE fp32 [batch, n_kv_head, >= max_kv_seq] or NULL */
+  int64_t weights_stride[2]; /* elements: batch, KV head */
+  int32_t batch, n_head, n_kv_head, max_kv_seq, head_dim;
+  int32_t window_size, n_sink; /* n_sink > 0 needs window_size > 0 */
+  int64_t q_stride[2];    /* elements: batch, head */
+  int64_t o_stride[2];
+  int64_t k_stride[3];    /* elements: page, KV head, row; multiples of 8 */
+  int64_t v_stride[3];
+  float scale;            /* <= 0 => 1/sqrt(head_dim) */
+  int32_t max_splits;     /* 0 => 64; clamped to [1,64] */
+  void* workspace;        /* DEVICE scratch, 16-byte aligned, private to the call until it has finished on its stream */
+  int64_t workspace_bytes;
+  int64_t total_kv_len;   /* as in TyrAttnDecodeArgs: steers the cut of the launch, results agree to rounding */
+} TyrAttnPagedDecodeArgs;
+
+/* Bytes of workspace the call below needs at most (0: none); looks at sizes, window_size, n_sink, max_splits and at
+ * whether `weights` is given.  Negative TYR_ATTN_ERR_* on bad sizes. */
+int64_t tyr_b200_attn_paged_decode_workspace_bytes(const TyrAttnPagedDecodeArgs* args);
+int tyr_b200_attn_paged_decode(const TyrAttnPagedDecodeArgs* args, void* stream);
+
+/* Brings the sequences of a paged cache back to a budget of n_keep keys by accumulated attention weight.  Per (sequence,
+ * KV head) of more than n_keep keys it keeps the first n_sink, the last n_recent and, of the others, the
+ * n_keep - n_sink - n_recent of greatest weight (of equal ones the lower position; a NaN ranks below every number),
+ * moves their K and V rows, in the order of their positions, to rows 0 .. n_keep - 1 of the sequence's own pages, moves
+ * their weights likewise and clears the weights from there to the sequence's old length.  Other rows stay as they
+ * are.  A sequence of at most n_keep keys keeps everything in place.  The sequences' pages must be their own: a
+ * page that two of them share would be moved under the other.
+ * kept[b, h, i] is the old position of key i, -1 behind a sequence's last.  new_lens must not be kv_lens.
+ * A length outside [0, max_kv_seq] is clamped and reported; a row whose page table entry is bad is not moved.
+ * Two launches. */
+typedef struct TyrAttnEvictArgs {
+  void* k; /* pools, 16-byte aligned */
+  void* v;
+  TyrAttnPageTable pages;
+  const int32_t* kv_lens; /* DEVICE int32 [batch] */
+  float* weights;         /* DEVICE fp32 [batch, n_kv_head, >= max_kv_seq] */
+  int64_t weights_stride[2];
+  int32_t* new_lens;      /* out, DEVICE int32 [batch]: min(length, n_keep) */
+  int32_t* kept;          /* out, DEVICE int32 [batch, n_kv_head, n_keep] contiguous */
+  int32_t batch, n_kv_head, max_kv_seq, head_dim; /* head_dim in {64,128,256} */
+  int32_t n_keep, n_recent, n_sink; /* n_keep > 0, n_recent + n_sink <= n_keep */
+  int64_t k_stride[3];    /* elements: page, KV head, row; multiples of 8 */
+  int64_t v_stride[3];
+} TyrAttnEvictArgs;
+
+int tyr_b200_attn_paged_evict(const TyrAttnEvictArgs* args, void* stream);
+
 /* LSE merge of two partial attention results over disjoint key sets (the
  * reduction Tyr states in ringAttnReduce, Tyr/GPU/Kernels/RingAttn.lean:164-180):
  *   L = Lr + log(1 + exp(Lb - Lr));  O = Or*exp(Lr-L) + Ob*exp(Lb-L).
@@ -283,6 +364,13 @@ typedef struct TyrAttnPrologueArgs {
 } TyrAttnPrologueArgs;
 
 int tyr_b200_attn_qk_prologue(const TyrAttnPrologueArgs* args, void* stream);
+/* The same into a paged cache: `out` is a pool, out_stride = {page, head, row}, `pages` says where the rows of batch
+ * element b lie; cap is ignored (max_pages * page_size rows) and out_at_row0 must be 0.  `rows`, DEVICE
+ * int32[batch] or NULL, gives the cache row of a sequence's first token where it is not its position (a cache that
+ * keys were evicted from); positions / position0 then select the rotary row only.  A row outside the table, or
+ * whose entry is bad, is skipped and reported. */
+int tyr_b200_attn_qk_prologue_paged(const TyrAttnPrologueArgs* args, const TyrAttnPageTable* pages, const int32_t* rows,
+                                    void* stream);
 
 /* ------------------------------------------------------------------------
  * Backward of the prefill operator: dQ, dK, dV from dO, the forward inputs, the

@@ -23,7 +23,8 @@ EXPORTS = [
     "tyr_b200_attn_prefill", "tyr_b200_attn_prefill_workspace_bytes", "tyr_b200_sdpa_4d", "tyr_b200_sdpa_gqa", "tyr_b200_sdpa_gqa_qkv",
     "tyr_b200_sdpa_gqa_window", "tyr_b200_sdpa_gqa_mask",
     "tyr_b200_attn_decode_workspace_bytes", "tyr_b200_attn_decode", "tyr_b200_attn_decode_static",
-    "tyr_b200_attn_merge", "tyr_b200_attn_qk_prologue",
+    "tyr_b200_attn_paged_decode_workspace_bytes", "tyr_b200_attn_paged_decode", "tyr_b200_attn_paged_evict",
+    "tyr_b200_attn_merge", "tyr_b200_attn_qk_prologue", "tyr_b200_attn_qk_prologue_paged",
     "tyr_b200_attn_backward_workspace_bytes", "tyr_b200_attn_backward",
     "tyr_b200_attn_prefill_host", "tyr_b200_attn_device_status", "tyr_b200_attn_device_check",
     "tyr_b200_attn_test_set_wait_limit", "tyr_b200_attn_test_stalled_wait", "tyr_b200_attn_strerror",
@@ -63,6 +64,29 @@ class PrologueArgs(ctypes.Structure):
         ("position0", c_i32), ("batch", c_i32), ("seq", c_i32), ("n_head", c_i32), ("head_dim", c_i32),
         ("x_stride", c_i64 * 3), ("out_stride", c_i64 * 3), ("eps", c_f32),
         ("cap", c_i32), ("max_pos", c_i32), ("pe", vp), ("pe_batch_stride", c_i64), ("out_at_row0", c_i32),
+    ]
+
+
+class PageTable(ctypes.Structure):
+    _fields_ = [("table", vp), ("table_stride", c_i64), ("max_pages", c_i32), ("n_pages", c_i32), ("page_size", c_i32)]
+
+
+class PagedDecodeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", vp), ("o", vp), ("lse", vp), ("k", vp), ("v", vp), ("pages", PageTable), ("kv_lens", vp),
+        ("weights", vp), ("weights_stride", c_i64 * 2),
+        ("batch", c_i32), ("n_head", c_i32), ("n_kv_head", c_i32), ("max_kv_seq", c_i32), ("head_dim", c_i32),
+        ("window_size", c_i32), ("n_sink", c_i32),
+        ("q_stride", c_i64 * 2), ("o_stride", c_i64 * 2), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3),
+        ("scale", c_f32), ("max_splits", c_i32), ("workspace", vp), ("workspace_bytes", c_i64), ("total_kv_len", c_i64),
+    ]
+
+
+class EvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("k", vp), ("v", vp), ("pages", PageTable), ("kv_lens", vp), ("weights", vp), ("weights_stride", c_i64 * 2),
+        ("new_lens", vp), ("kept", vp), ("batch", c_i32), ("n_kv_head", c_i32), ("max_kv_seq", c_i32), ("head_dim", c_i32),
+        ("n_keep", c_i32), ("n_recent", c_i32), ("n_sink", c_i32), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3),
     ]
 
 
@@ -118,6 +142,14 @@ def load() -> ctypes.CDLL:
     L.tyr_b200_attn_decode_static.restype = ctypes.c_int
     L.tyr_b200_attn_qk_prologue.argtypes = [ctypes.POINTER(PrologueArgs), vp]
     L.tyr_b200_attn_qk_prologue.restype = ctypes.c_int
+    L.tyr_b200_attn_paged_decode_workspace_bytes.argtypes = [ctypes.POINTER(PagedDecodeArgs)]
+    L.tyr_b200_attn_paged_decode_workspace_bytes.restype = c_i64
+    L.tyr_b200_attn_paged_decode.argtypes = [ctypes.POINTER(PagedDecodeArgs), vp]
+    L.tyr_b200_attn_paged_decode.restype = ctypes.c_int
+    L.tyr_b200_attn_paged_evict.argtypes = [ctypes.POINTER(EvictArgs), vp]
+    L.tyr_b200_attn_paged_evict.restype = ctypes.c_int
+    L.tyr_b200_attn_qk_prologue_paged.argtypes = [ctypes.POINTER(PrologueArgs), ctypes.POINTER(PageTable), vp, vp]
+    L.tyr_b200_attn_qk_prologue_paged.restype = ctypes.c_int
     L.tyr_b200_attn_backward_workspace_bytes.argtypes = [c_i32] * 3
     L.tyr_b200_attn_backward_workspace_bytes.restype = c_u64
     L.tyr_b200_attn_backward.argtypes = [ctypes.POINTER(BackwardArgs), vp]

@@ -14,8 +14,8 @@ LIB_PATH = os.path.join(LIB_DIR, "libtyr_b200_attn.so")
 CALLS_PATH = os.path.join(LIB_DIR, "_calls.so")   # the Python call layer: a CPython extension over the C ABI
 CALLS_SOURCE = "py_calls.cpp"
 SOURCES = ["api.cu", "prefill_sm100.cu", "backward_sm100.cu", "decode_splitkv.cu", "check_fp32.cu", "qk_prologue.cu",
-           "stalled_wait.cu"]
-HEADERS = ["ptx_sm100.cuh", "mma_sync.cuh", "attn_internal.h", "scan_plan.h", "unit_parts.h",
+           "paged_evict.cu", "stalled_wait.cu"]
+HEADERS = ["ptx_sm100.cuh", "mma_sync.cuh", "attn_internal.h", "scan_plan.h", "unit_parts.h", "fast_div.h",
            os.path.join("..", "..", "include", "tyr_b200_attn.h")]
 
 # The reference's own nvcc flags for GPU=B200 (cc/Makefile:66-76) minus fast-math

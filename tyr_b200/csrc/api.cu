@@ -129,6 +129,31 @@ int check_prefill(const TyrAttnPrefillArgs* a) {
   return 0;
 }
 
+// ---- paged cache
+int check_page_table(const TyrAttnPageTable& t, int64_t max_kv_seq) {
+  if (t.max_pages <= 0 || t.n_pages <= 0 || t.page_size <= 0 || t.table_stride < 0) return -TYR_ATTN_ERR_SHAPE;
+  const int64_t cap = (int64_t)t.max_pages * t.page_size;
+  if (cap > 0x7fffffffLL) return -TYR_ATTN_ERR_TOO_LARGE;
+  return max_kv_seq > cap ? -TYR_ATTN_ERR_RANGE : 0;  // a sequence may not reach behind its row of the table
+}
+// rows are read and written with 16-byte accesses
+bool pool_aligned(const void* pool, const int64_t* stride) {
+  return aligned16(pool) && !((stride[0] | stride[1] | stride[2]) & 7) && stride[2] > 0 && stride[0] >= 0 && stride[1] >= 0;
+}
+// the (sequence, KV head) rows of the running sums are written by different CTAs: they may not overlap
+bool sums_apart(const int64_t* stride, int batch, int n_kv_head, int max_kv_seq) {
+  return (batch == 1 || stride[0] >= max_kv_seq) && (n_kv_head == 1 || stride[1] >= max_kv_seq);
+}
+int check_paged_decode_sizes(const TyrAttnPagedDecodeArgs* a) {
+  if (!a) return -TYR_ATTN_ERR_NULL;
+  if (a->batch <= 0 || a->n_head <= 0 || a->n_kv_head <= 0 || a->max_kv_seq <= 0) return -TYR_ATTN_ERR_SHAPE;
+  if (a->n_head % a->n_kv_head != 0) return -TYR_ATTN_ERR_SHAPE;
+  if (a->window_size < 0 || a->n_sink < 0 || (a->n_sink > 0 && a->window_size == 0)) return -TYR_ATTN_ERR_SHAPE;
+  if (a->head_dim != 64 && a->head_dim != 128) return -TYR_ATTN_ERR_HEAD_DIM;
+  if (a->batch > 65535 || a->n_kv_head > 65535) return -TYR_ATTN_ERR_TOO_LARGE;
+  return 0;
+}
+
 void contiguous_strides(int64_t* s, int64_t heads, int64_t seq, int64_t d) {
   s[2] = d;
   s[1] = seq * d;
@@ -280,6 +305,52 @@ int tyr_b200_attn_decode(const TyrAttnDecodeArgs* a, void* stream) {
   return launch_decode(*a, scale, static_cast<cudaStream_t>(stream));
 }
 
+int64_t tyr_b200_attn_paged_decode_workspace_bytes(const TyrAttnPagedDecodeArgs* a) {
+  const int rc = check_paged_decode_sizes(a);
+  return rc ? rc : (int64_t)paged_decode_workspace_bytes(*a);
+}
+
+int tyr_b200_attn_paged_decode(const TyrAttnPagedDecodeArgs* a, void* stream) {
+  if (a && a->batch == 0 && a->n_head >= 0 && a->n_kv_head >= 0 && a->head_dim > 0) return 0;  // no sequence: nothing to do
+  if (!a || !a->q || !a->o || !a->k || !a->v || !a->pages.table || !a->kv_lens) return -TYR_ATTN_ERR_NULL;
+  int rc = check_paged_decode_sizes(a);
+  if (rc) return rc;
+  if ((rc = check_page_table(a->pages, a->max_kv_seq))) return rc;
+  if (!pool_aligned(a->k, a->k_stride) || !pool_aligned(a->v, a->v_stride)) return -TYR_ATTN_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(a->q) & 3u) || (a->q_stride[0] & 1) || (a->q_stride[1] & 1) ||
+      (reinterpret_cast<uintptr_t>(a->o) & 1u))
+    return -TYR_ATTN_ERR_ALIGN;
+  if (a->weights && !sums_apart(a->weights_stride, a->batch, a->n_kv_head, a->max_kv_seq)) return -TYR_ATTN_ERR_SHAPE;
+  if (a->weights && (reinterpret_cast<uintptr_t>(a->weights) & 3u)) return -TYR_ATTN_ERR_ALIGN;
+  const size_t need = paged_decode_workspace_bytes(*a);
+  if (need > 0 && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < (int64_t)need)) return -TYR_ATTN_ERR_WORKSPACE;
+  int dev = 0;
+  if ((rc = current_device_checked(&dev))) return rc;
+  DeviceState* ds = device_state(dev);
+  if (!ds) return -TYR_ATTN_ERR_NO_DEVICE;
+  return launch_paged_decode(*a, resolve_scale(a->scale, a->head_dim), ds->status, static_cast<cudaStream_t>(stream));
+}
+
+int tyr_b200_attn_paged_evict(const TyrAttnEvictArgs* a, void* stream) {
+  if (a && a->batch == 0 && a->n_kv_head >= 0 && a->head_dim > 0) return 0;
+  if (!a || !a->k || !a->v || !a->pages.table || !a->kv_lens || !a->weights || !a->new_lens || !a->kept) return -TYR_ATTN_ERR_NULL;
+  if (a->batch <= 0 || a->n_kv_head <= 0 || a->max_kv_seq <= 0) return -TYR_ATTN_ERR_SHAPE;
+  if (a->n_keep <= 0 || a->n_recent < 0 || a->n_sink < 0 || (int64_t)a->n_recent + a->n_sink > a->n_keep) return -TYR_ATTN_ERR_SHAPE;
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return -TYR_ATTN_ERR_HEAD_DIM;
+  if (a->batch > 65535 || a->n_kv_head > 65535) return -TYR_ATTN_ERR_TOO_LARGE;
+  if (!sums_apart(a->weights_stride, a->batch, a->n_kv_head, a->max_kv_seq)) return -TYR_ATTN_ERR_SHAPE;
+  if (a->batch > 1 && a->pages.table_stride == 0) return -TYR_ATTN_ERR_SHAPE;  // one row of the table for all: shared pages
+  if (a->new_lens == a->kv_lens) return -TYR_ATTN_ERR_SHAPE;  // the lengths are read until the last row has moved
+  int rc = check_page_table(a->pages, a->max_kv_seq);
+  if (rc) return rc;
+  if (!pool_aligned(a->k, a->k_stride) || !pool_aligned(a->v, a->v_stride)) return -TYR_ATTN_ERR_ALIGN;
+  int dev = 0;
+  if ((rc = current_device_checked(&dev))) return rc;
+  DeviceState* ds = device_state(dev);
+  if (!ds) return -TYR_ATTN_ERR_NO_DEVICE;
+  return launch_paged_evict(*a, ds->status, static_cast<cudaStream_t>(stream));
+}
+
 int tyr_b200_attn_merge(const float* o_a, const float* lse_a, const float* o_b, const float* lse_b,
                         float* o_out, float* lse_out, int64_t rows, int32_t head_dim, void* stream) {
   if (!o_a || !lse_a || !o_b || !lse_b || !o_out || !lse_out) return -TYR_ATTN_ERR_NULL;
@@ -288,7 +359,7 @@ int tyr_b200_attn_merge(const float* o_a, const float* lse_a, const float* o_b, 
                        static_cast<cudaStream_t>(stream));
 }
 
-int tyr_b200_attn_qk_prologue(const TyrAttnPrologueArgs* a, void* stream) {
+static int qk_prologue(const TyrAttnPrologueArgs* a, const TyrAttnPageTable* pages, const int32_t* rows, void* stream) {
   if (!a || !a->x || !a->out) return -TYR_ATTN_ERR_NULL;
   if ((a->cos == nullptr) != (a->sin == nullptr)) return -TYR_ATTN_ERR_NULL;
   if (a->pe && a->cos) return -TYR_ATTN_ERR_SHAPE;  // one rotary form per call
@@ -296,10 +367,17 @@ int tyr_b200_attn_qk_prologue(const TyrAttnPrologueArgs* a, void* stream) {
   if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return -TYR_ATTN_ERR_HEAD_DIM;
   // every written row and every rotary row must exist: the reference guards its append with
   // `cache.seq < cache.maxLen` (Tyr/Model/Qwen/Attention.lean:189)
-  if (a->cap <= 0 || ((a->cos || a->pe) && a->max_pos <= 0)) return -TYR_ATTN_ERR_SHAPE;
-  if (a->out_at_row0 && a->seq > a->cap) return -TYR_ATTN_ERR_RANGE;
+  int64_t cap = a->cap;
+  if (pages) {
+    const int rc = check_page_table(*pages, 0);
+    if (rc) return rc;
+    if (a->out_at_row0) return -TYR_ATTN_ERR_SHAPE;
+    cap = (int64_t)pages->max_pages * pages->page_size;
+  }
+  if (cap <= 0 || ((a->cos || a->pe) && a->max_pos <= 0)) return -TYR_ATTN_ERR_SHAPE;
+  if (a->out_at_row0 && a->seq > cap) return -TYR_ATTN_ERR_RANGE;
   if (!a->positions) {
-    if (!a->out_at_row0 && (int64_t)a->position0 + a->seq > a->cap) return -TYR_ATTN_ERR_RANGE;
+    if (!a->out_at_row0 && !rows && (int64_t)a->position0 + a->seq > cap) return -TYR_ATTN_ERR_RANGE;
     if ((a->cos || a->pe) && (int64_t)a->position0 + a->seq > a->max_pos) return -TYR_ATTN_ERR_RANGE;
   }
   if (!aligned16(a->x) || !aligned16(a->out) || (a->norm_weight && !aligned16(a->norm_weight)) ||
@@ -312,7 +390,14 @@ int tyr_b200_attn_qk_prologue(const TyrAttnPrologueArgs* a, void* stream) {
   if ((rc = current_device_checked(&dev))) return rc;
   DeviceState* ds = device_state(dev);
   if (!ds) return -TYR_ATTN_ERR_NO_DEVICE;
-  return launch_qk_prologue(*a, ds->status, static_cast<cudaStream_t>(stream));
+  return launch_qk_prologue(*a, pages, rows, ds->status, static_cast<cudaStream_t>(stream));
+}
+
+int tyr_b200_attn_qk_prologue(const TyrAttnPrologueArgs* a, void* stream) { return qk_prologue(a, nullptr, nullptr, stream); }
+
+int tyr_b200_attn_qk_prologue_paged(const TyrAttnPrologueArgs* a, const TyrAttnPageTable* pages, const int32_t* rows, void* stream) {
+  if (!pages || !pages->table) return -TYR_ATTN_ERR_NULL;
+  return qk_prologue(a, pages, rows, stream);
 }
 
 uint64_t tyr_b200_attn_backward_workspace_bytes(int32_t batch, int32_t n_head, int32_t q_seq) {

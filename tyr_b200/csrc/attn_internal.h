@@ -80,6 +80,8 @@ int launch_prefill_check(const TyrAttnPrefillArgs& a, float scale, cudaStream_t 
 size_t decode_workspace_bytes(int batch, int n_head, int head_dim, int max_kv_seq, int max_splits);
 int decode_num_splits(int max_kv_seq, int max_splits, int* chunk_len);
 int launch_decode(const TyrAttnDecodeArgs& a, float scale, cudaStream_t st);
+size_t paged_decode_workspace_bytes(const TyrAttnPagedDecodeArgs& a);
+int launch_paged_decode(const TyrAttnPagedDecodeArgs& a, float scale, int* status, cudaStream_t st);
 // Unmasked forward calls with few query rows per KV head (group * q_seq), served by the decode kernel.
 bool few_rows_call(const TyrAttnPrefillArgs& a);
 size_t few_rows_workspace_bytes(const TyrAttnPrefillArgs& a);  // 0: the launch would not use one
@@ -88,6 +90,10 @@ int launch_merge2(const float* o_a, const float* lse_a, const float* o_b, const 
                   float* o_out, float* lse_out, int64_t rows, int head_dim, cudaStream_t st);
 
 // qk_prologue.cu
-int launch_qk_prologue(const TyrAttnPrologueArgs& a, int* status, cudaStream_t st);
+// `pages` null: into a dense tensor
+int launch_qk_prologue(const TyrAttnPrologueArgs& a, const TyrAttnPageTable* pages, const int32_t* rows, int* status,
+                       cudaStream_t st);
+// paged_evict.cu
+int launch_paged_evict(const TyrAttnEvictArgs& a, int* status, cudaStream_t st);
 
 }  // namespace tyr

@@ -29,8 +29,10 @@
 #include <algorithm>
 #include <atomic>
 #include <mutex>
+#include <type_traits>
 
 #include "attn_internal.h"
+#include "fast_div.h"
 #include "mma_sync.cuh"
 #include "ptx_sm100.cuh"
 #include "scan_plan.h"
@@ -67,6 +69,29 @@ struct DecodeParams {
   int* status;    // per-device status word (out-of-range lengths are reported there)
 };
 
+// A cache in pages (tyr_b200_attn_paged_decode).  The query sees the first `n_sink` and the last `window` keys (all of them
+// with window = 0); everything below counts the VISIBLE keys, 0 .. n_visible - 1, max_kv_seq being the most a
+// sequence can have of them, so that no step is spent on keys out of sight: visible key v is key v of the sequence
+// among the first ones and key v + gap behind them.
+struct PagedParams : DecodeParams {
+  const int32_t* table;
+  int64_t table_stride;
+  FastDiv by_page;
+  int n_pages, max_len, window, n_sink;
+  float* ws_scores;   // [batch, n_head, max_kv_seq] scores in the log2 domain, for the running sums of the weights; or null
+};
+template <class P>
+constexpr bool kIsPaged = std::is_same<P, PagedParams>::value;
+
+struct Visible {
+  int n, first, gap;   // visible keys; how many of them are first tokens; keys out of sight behind those
+};
+__device__ __forceinline__ Visible visible_of(int len, const PagedParams& p) {
+  const int begin = p.window > 0 ? max(len - p.window, 0) : 0;
+  const int first = min(p.n_sink, begin);
+  return {len - begin + first, first, begin - first};
+}
+
 // Row `r` of the KV head's rows (query head and query row) in O and in the LSE array.
 __device__ __forceinline__ __nv_bfloat16* o_row(const DecodeParams& p, int b, int hkv, int r) {
   const int h = r / p.q_seq, i = r - h * p.q_seq;
@@ -101,6 +126,24 @@ __device__ __noinline__ int bad_length(int raw, const DecodeParams& p, int b, in
   return len;
 }
 
+// The paged call's lengths: 0 is an idle slot, whose rows are zeros with LSE = -inf; one outside [0, max_len] is clamped
+// and reported.  Out of line, as above.
+template <int D>
+__device__ __noinline__ int paged_odd_length(int raw, const PagedParams& p, int b, int hkv, int row0, int rows_here) {
+  const int len = min(max(raw, 0), p.max_len);
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0 && hkv == 0 && row0 == 0 && raw != len) atomicOr(p.status, kStatusOutOfRange);
+    if (len == 0) {
+      for (int idx = threadIdx.x; idx < rows_here * D; idx += blockDim.x) {
+        const int r = row0 + idx / D, d = idx % D;
+        o_row(p, b, hkv, r)[d] = __float2bfloat16_rn(0.f);
+        if (d == 0 && p.lse) p.lse[lse_index(p, b, hkv, r)] = -INFINITY;
+      }
+    }
+  }
+  return len;
+}
+
 template <int D, int kWarps, int kNT>
 struct DCfg {
   static constexpr int kRows = 8 * kNT;                 // query rows of a CTA, in column tiles of 8
@@ -121,10 +164,12 @@ struct DCfg {
 
 // kCluster: the grid's x extent is one cluster, its CTAs cut the sequence's keys evenly and merge among
 // themselves; no workspace, no second launch.  Otherwise chunks of p.chunk_len keys, partials to the workspace.
-template <int D, int kWarps, int kNT, bool kCluster>
+// P: DecodeParams for the dense and ragged caches, PagedParams for the paged one.
+template <int D, int kWarps, int kNT, bool kCluster, class P>
 __global__ void __launch_bounds__(32 * kWarps)
-decode_kernel(const __grid_constant__ DecodeParams p) {
+decode_kernel(const __grid_constant__ P p) {
   using C = DCfg<D, kWarps, kNT>;
+  constexpr bool kPaged = kIsPaged<P>;
   constexpr int kThreads = C::kThreads, kTileKeys = C::kTileKeys, kRows = C::kRows;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t sbase = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
@@ -137,7 +182,14 @@ decode_kernel(const __grid_constant__ DecodeParams p) {
   const int rows_here = min(kRows, p.rows - row0);
   const int b = blockIdx.z;
   int len = p.kv_lens ? p.kv_lens[b] : p.max_kv_seq;
-  if (len <= 0 || len > p.max_kv_seq) len = bad_length<D>(len, p, b, hkv, row0, rows_here);
+  Visible vis{0, 0, 0};
+  if constexpr (kPaged) {
+    if (len <= 0 || len > p.max_len) len = paged_odd_length<D>(len, p, b, hkv, row0, rows_here);
+    vis = visible_of(len, p);
+    len = vis.n;
+  } else {
+    if (len <= 0 || len > p.max_kv_seq) len = bad_length<D>(len, p, b, hkv, row0, rows_here);
+  }
   if (kCluster && len == 0) return;  // the whole cluster: its CTAs share the sequence
   int chunk_len = p.chunk_len;
   if (kCluster) chunk_len = ((len + p.n_splits - 1) / p.n_splits + kWarpKeys - 1) / kWarpKeys * kWarpKeys;
@@ -148,7 +200,10 @@ decode_kernel(const __grid_constant__ DecodeParams p) {
   const int n_tiles = max(key_end - key_begin + kTileKeys - 1, 0) / kTileKeys;  // 0: a CTA of the cluster without keys
 
   const __nv_bfloat16 *kbase, *vbase;
-  if (p.k_ptrs) {
+  if constexpr (kPaged) {
+    kbase = p.k + hkv * p.ks[1];
+    vbase = p.v + hkv * p.vs[1];
+  } else if (p.k_ptrs) {
     const int64_t hs_k = p.kv_head_strides ? p.kv_head_strides[b] : (int64_t)len * p.ks[2];
     const int64_t hs_v = p.kv_head_strides ? p.kv_head_strides[b] : (int64_t)len * p.vs[2];
     kbase = static_cast<const __nv_bfloat16*>(p.k_ptrs[b]) + hkv * hs_k;
@@ -161,24 +216,64 @@ decode_kernel(const __grid_constant__ DecodeParams p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int quad = lane >> 2, t4 = lane & 3;
 
+  // ---- paged cache: where the rows of a tile lie.  The kLoads rows a thread loads a piece of are the same for the
+  // kChunksPerRow lanes of its group, so each lane looks one of them up, a tile ahead of the loads, and the lanes
+  // exchange what they found: a table entry's latency is not on the path of the loads.
+  constexpr int kLoads = kTileKeys * C::kChunksPerRow / kThreads, kRowStep = kThreads / C::kChunksPerRow;
+  struct Where { int page, row; };
+  bool bad_page = false;
+  auto look_up = [&](int tile) {
+    Where w{0, 0};
+    if constexpr (kPaged) {
+      const int kr = (lane % C::kChunksPerRow) % kLoads * kRowStep + tid / C::kChunksPerRow;
+      const int v = min(key_begin + tile * kTileKeys + kr, key_end - 1);
+      const int key = v + (v >= vis.first ? vis.gap : 0);
+      const int at = p.by_page.div(key);
+      w.row = key - at * (int)p.by_page.d;
+      w.page = p.table[b * p.table_stride + at];
+      if ((unsigned)w.page >= (unsigned)p.n_pages) {  // not followed
+        bad_page = true;
+        w.page = 0;
+      }
+    }
+    return w;
+  };
+
   // ---- stage loader: kTileKeys keys x D bf16 of K and of V, 16 bytes per cp.async
-  auto load_tile = [&](int tile, int stage) {
+  auto load_tile = [&](int tile, int stage, Where where) {
     const uint32_t sk = sbase + stage * C::kStageBytes, sv = sk + C::kTileBytes;
     const int k0 = key_begin + tile * kTileKeys;
 #pragma unroll
-    for (int it = 0; it < kTileKeys * C::kChunksPerRow / kThreads; ++it) {
+    for (int it = 0; it < kLoads; ++it) {
       const int idx = it * kThreads + tid;
       const int kr = idx / C::kChunksPerRow, c = idx % C::kChunksPerRow;
+      if constexpr (kPaged) {
+        const int64_t page = __shfl_sync(0xffffffffu, where.page, it, C::kChunksPerRow);
+        const int64_t row = __shfl_sync(0xffffffffu, where.row, it, C::kChunksPerRow);
+        cp_async16(sk + sw_off<D>(kr, c), kbase + page * p.ks[0] + row * p.ks[2] + c * 8);
+        cp_async16(sv + sw_off<D>(kr, c), vbase + page * p.vs[0] + row * p.vs[2] + c * 8);
+        continue;
+      }
       const int key = min(k0 + kr, key_end - 1);  // rows past the end re-read the last valid key
       cp_async16(sk + sw_off<D>(kr, c), kbase + (int64_t)key * p.ks[2] + c * 8);
       cp_async16(sv + sw_off<D>(kr, c), vbase + (int64_t)key * p.vs[2] + c * 8);
     }
   };
 
+  Where ahead[kStages - 1] = {};
+  if constexpr (kPaged) {
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s)
+      if (s < n_tiles) ahead[s] = look_up(s);
+  }
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
-    if (s < n_tiles) load_tile(s, s);
+    if (s < n_tiles) load_tile(s, s, ahead[s]);
     cp_async_commit();
+  }
+  Where next{0, 0};
+  if constexpr (kPaged) {
+    if (kStages - 1 < n_tiles) next = look_up(kStages - 1);
   }
 
   // ---- Q fragments (B operand: column = query row of this KV head)
@@ -210,8 +305,11 @@ decode_kernel(const __grid_constant__ DecodeParams p) {
   for (int tile = 0; tile < n_tiles; ++tile) {
     cp_async_wait<kStages - 2>();
     __syncthreads();
-    if (tile + kStages - 1 < n_tiles) load_tile(tile + kStages - 1, (tile + kStages - 1) % kStages);
+    if (tile + kStages - 1 < n_tiles) load_tile(tile + kStages - 1, (tile + kStages - 1) % kStages, next);
     cp_async_commit();
+    if constexpr (kPaged) {
+      if (tile + kStages < n_tiles) next = look_up(tile + kStages);
+    }
 
     const int stage = tile % kStages;
     const uint32_t sk = sbase + stage * C::kStageBytes, sv = sk + C::kTileBytes;
@@ -245,6 +343,19 @@ decode_kernel(const __grid_constant__ DecodeParams p) {
         sx[nt][2 + x] = live1 ? (sacc[nt][0][2 + x] + sacc[nt][1][2 + x]) * p.scale_log2 : -INFINITY;
         mx[nt][x] = fmaxf(sx[nt][x], sx[nt][2 + x]);
       }
+    if constexpr (kPaged) {
+      if (p.ws_scores != nullptr) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int r = nt * 8 + 2 * t4 + x;
+            float* to = p.ws_scores + lse_index(p, b, hkv, row0 + r) * p.max_kv_seq + gkey0 + quad;
+            if (r < rows_here && live0) to[0] = sx[nt][x];
+            if (r < rows_here && live1) to[8] = sx[nt][2 + x];
+          }
+      }
+    }
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1)
 #pragma unroll
@@ -305,7 +416,16 @@ decode_kernel(const __grid_constant__ DecodeParams p) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) l_run[nt][x] += __shfl_xor_sync(0xffffffffu, l_run[nt][x], o);
   cp_async_wait<0>();
-  __syncthreads();
+  if constexpr (kPaged) {
+    // a key that is not where the table says has no value: the rows of this KV head become NaN
+    if (bad_page) atomicOr(p.status, kStatusOutOfRange);
+    if (__syncthreads_or(bad_page)) {
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) l_run[nt][0] = l_run[nt][1] = __int_as_float(0x7fffffff);
+    }
+  } else {
+    __syncthreads();
+  }
   constexpr int kMS = C::kMergeStride;
   float* sc_o = reinterpret_cast<float*>(smem);               // [warps][rows][D + 4]
   float* sc_ml = sc_o + kWarps * kRows * kMS;                 // [warps][rows][2]
@@ -407,16 +527,18 @@ decode_kernel(const __grid_constant__ DecodeParams p) {
 // Launched with programmatic stream serialisation: its CTAs may become resident while the split
 // kernel is still draining, and wait here until that grid has completed and its writes are visible,
 // so the launch latency of this second kernel hides behind the tail of the first.
-template <int D>
+template <int D, class P>
 __global__ void __launch_bounds__(kMergeThreads)
-decode_merge_kernel(const DecodeParams p) {
+decode_merge_kernel(const P p) {
   constexpr int kLanes = D / 4, kGroups = kMergeThreads / kLanes;
   __shared__ float4 s_acc[kGroups][kLanes];
   __shared__ float s_w[kGroups];
   grid_launch_dependents();
   grid_dependency_wait();
   const int row = blockIdx.x, b = blockIdx.y;  // row of the sequence: head * q_seq + query
-  const int len = p.kv_lens ? min(max(p.kv_lens[b], 0), p.max_kv_seq) : p.max_kv_seq;
+  int len;
+  if constexpr (kIsPaged<P>) len = visible_of(min(max(p.kv_lens[b], 0), p.max_len), p).n;
+  else len = p.kv_lens ? min(max(p.kv_lens[b], 0), p.max_kv_seq) : p.max_kv_seq;
   const int n_chunks = (len + p.chunk_len - 1) / p.chunk_len;
   if (n_chunks <= 1) return;  // the split kernel already wrote the final row
   const int g = threadIdx.x / kLanes, l = threadIdx.x % kLanes, lane = threadIdx.x & 31;
@@ -465,6 +587,29 @@ decode_merge_kernel(const DecodeParams p) {
   }
 }
 
+// Running sums of the weights: weights[b, hkv, key] += sum over the group's heads of 2^(score - lse).  The scores are those
+// the split kernel left in the workspace: 4 bytes per key and query head, where forming them again would read the key's
+// 2 D bytes a second time.  One thread per visible key, the group's heads in order: no atomics.
+constexpr int kSumThreads = 256;
+__global__ void __launch_bounds__(kSumThreads)
+weight_sums_kernel(const PagedParams p, float* weights, int64_t stride_b, int64_t stride_h) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int hkv = blockIdx.y, b = blockIdx.z;
+  const Visible vis = visible_of(min(max(p.kv_lens[b], 0), p.max_len), p);
+  const int v = blockIdx.x * kSumThreads + threadIdx.x;
+  if (v >= vis.n) return;
+  float acc = 0.f;
+  for (int r = 0; r < p.rows; ++r) {
+    const int64_t at = lse_index(p, b, hkv, r);
+    const float lse = p.lse[at];
+    // (a row without any weight, every score -inf, gives none)
+    acc += lse == -INFINITY ? 0.f : ex2f(p.ws_scores[at * p.max_kv_seq + v] - lse * kLog2e);
+  }
+  float* w = weights + b * stride_b + hkv * stride_h + v + (v >= vis.first ? vis.gap : 0);
+  *w += acc;
+}
+
 // Two-way merge, natural-log LSE (the formula of RingAttn.lean:164-180).
 __global__ void merge2_kernel(const float* o_a, const float* lse_a, const float* o_b,
                               const float* lse_b, float* o_out, float* lse_out, int64_t rows, int d) {
@@ -480,8 +625,8 @@ __global__ void merge2_kernel(const float* o_a, const float* lse_a, const float*
   if (threadIdx.x == 0) lse_out[r] = L;
 }
 
-template <int D, int kWarps, int kNT, bool kCluster>
-cudaError_t launch_scan(const DecodeParams& p, cudaStream_t st) {
+template <int D, int kWarps, int kNT, bool kCluster, class P>
+cudaError_t launch_scan(const P& p, cudaStream_t st) {
   constexpr int kSmem = DCfg<D, kWarps, kNT>::kSmemBytes;
   static std::atomic<bool> attr_set[64] = {};  // per device
   int dev = 0;
@@ -489,32 +634,32 @@ cudaError_t launch_scan(const DecodeParams& p, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!attr_set[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(decode_kernel<D, kWarps, kNT, kCluster>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    e = cudaFuncSetAttribute(decode_kernel<D, kWarps, kNT, kCluster, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e == cudaSuccess && kCluster)
-      e = cudaFuncSetAttribute(decode_kernel<D, kWarps, kNT, kCluster>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      e = cudaFuncSetAttribute(decode_kernel<D, kWarps, kNT, kCluster, P>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     attr_set[dev].store(true, std::memory_order_release);
   }
-  return launch_overlapped(decode_kernel<D, kWarps, kNT, kCluster>, dim3(p.n_splits, p.n_kv_head * p.row_groups, p.batch), dim3(32 * kWarps),
+  return launch_overlapped(decode_kernel<D, kWarps, kNT, kCluster, P>, dim3(p.n_splits, p.n_kv_head * p.row_groups, p.batch), dim3(32 * kWarps),
                            kSmem, st, kCluster ? p.n_splits : 1, p);
 }
 
-template <int D, int kNT>
-cudaError_t launch_scan_of(const DecodeParams& p, const ScanPlan& s, cudaStream_t st) {
-  if (s.cluster) return s.warps == 8 ? launch_scan<D, 8, kNT, true>(p, st) : launch_scan<D, 4, kNT, true>(p, st);
-  return s.warps == 8 ? launch_scan<D, 8, kNT, false>(p, st) : launch_scan<D, 4, kNT, false>(p, st);
+template <int D, int kNT, class P>
+cudaError_t launch_scan_of(const P& p, const ScanPlan& s, cudaStream_t st) {
+  if (s.cluster) return s.warps == 8 ? launch_scan<D, 8, kNT, true, P>(p, st) : launch_scan<D, 4, kNT, true, P>(p, st);
+  return s.warps == 8 ? launch_scan<D, 8, kNT, false, P>(p, st) : launch_scan<D, 4, kNT, false, P>(p, st);
 }
 
-template <int D>
-int launch_d(DecodeParams& p, const ScanPlan& s, cudaStream_t st) {
+template <int D, class P>
+int launch_d(P& p, const ScanPlan& s, cudaStream_t st) {
   if (!s.covers(p.max_kv_seq)) return -TYR_ATTN_ERR_SHAPE;  // (the kernel divides by the chunk length)
   p.n_splits = s.n_splits;
   p.chunk_len = s.chunk_len;
-  cudaError_t e = p.rows <= 8 ? launch_scan_of<D, 1>(p, s, st) : launch_scan_of<D, 2>(p, s, st);
+  cudaError_t e = p.rows <= 8 ? launch_scan_of<D, 1, P>(p, s, st) : launch_scan_of<D, 2, P>(p, s, st);
   count_launch();
   if (e != cudaSuccess) return (int)e;
   if (s.needs_workspace()) {
-    e = launch_overlapped(decode_merge_kernel<D>, dim3(p.n_head * p.q_seq, p.batch), dim3(kMergeThreads), 0, st, 1, p);
+    e = launch_overlapped(decode_merge_kernel<D, P>, dim3(p.n_head * p.q_seq, p.batch), dim3(kMergeThreads), 0, st, 1, p);
     count_launch();
   }
   return (int)(e != cudaSuccess ? e : cudaGetLastError());
@@ -635,6 +780,71 @@ int launch_decode(const TyrAttnDecodeArgs& a, float scale, cudaStream_t st) {
   if (a.head_dim == 128) return launch_d<128>(p, s, st);
   if (a.head_dim == 64) return launch_d<64>(p, s, st);
   return -TYR_ATTN_ERR_HEAD_DIM;
+}
+
+// ---- paged cache
+static int most_visible(const TyrAttnPagedDecodeArgs& a) {
+  return a.window_size > 0 ? (int)std::min<long long>(a.max_kv_seq, (long long)a.window_size + a.n_sink) : a.max_kv_seq;
+}
+// workspace: partial rows and their LSEs, then, for the sums of the weights, every score and the rows' LSEs
+static size_t paged_partial_bytes(const TyrAttnPagedDecodeArgs& a) {
+  return (decode_workspace_bytes(a.batch, a.n_head, a.head_dim, most_visible(a), a.max_splits) + 255) & ~(size_t)255;
+}
+size_t paged_decode_workspace_bytes(const TyrAttnPagedDecodeArgs& a) {
+  const size_t rows = (size_t)a.batch * a.n_head;
+  return paged_partial_bytes(a) + (a.weights ? rows * ((size_t)most_visible(a) + 1) * sizeof(float) : 0);
+}
+
+int launch_paged_decode(const TyrAttnPagedDecodeArgs& a, float scale, int* status, cudaStream_t st) {
+  PagedParams p;
+  p.q = static_cast<const __nv_bfloat16*>(a.q);
+  p.o = static_cast<__nv_bfloat16*>(a.o);
+  p.lse = a.lse;
+  p.k = static_cast<const __nv_bfloat16*>(a.k);
+  p.v = static_cast<const __nv_bfloat16*>(a.v);
+  p.k_ptrs = p.v_ptrs = nullptr;
+  p.kv_lens = a.kv_lens;
+  p.kv_head_strides = nullptr;
+  p.batch = a.batch; p.n_head = a.n_head; p.n_kv_head = a.n_kv_head; p.max_kv_seq = most_visible(a);
+  p.q_seq = 1;
+  p.rows = a.n_head / a.n_kv_head;
+  p.row_groups = (p.rows + 15) / 16;
+  for (int i = 0; i < 2; ++i) { p.qs[i] = a.q_stride[i]; p.os[i] = a.o_stride[i]; }
+  p.qs[2] = p.os[2] = 0;
+  for (int i = 0; i < 3; ++i) { p.ks[i] = a.k_stride[i]; p.vs[i] = a.v_stride[i]; }
+  p.scale_log2 = scale * kLog2e;
+  p.status = status;
+  p.table = a.pages.table;
+  p.table_stride = a.pages.table_stride;
+  p.by_page = make_fastdiv(a.pages.page_size);
+  p.n_pages = a.pages.n_pages;
+  p.max_len = a.max_kv_seq;
+  p.window = a.window_size;
+  p.n_sink = a.n_sink;
+  if ((long long)p.n_kv_head * p.row_groups > 65535) return -TYR_ATTN_ERR_TOO_LARGE;  // (the grid's y extent)
+  char* ws = static_cast<char*>(a.workspace);
+  p.ws_o = reinterpret_cast<float*>(ws);
+  p.ws_lse = nullptr;
+  p.ws_aligned = 1;
+  p.ws_scores = nullptr;
+  if (a.weights) {
+    p.ws_scores = reinterpret_cast<float*>(ws + paged_partial_bytes(a));
+    if (!p.lse) p.lse = p.ws_scores + (size_t)a.batch * a.n_head * p.max_kv_seq;
+  }
+  ScanPlan s;
+  s.n_splits = decode_launch_splits(p.max_kv_seq, a.max_splits, a.batch, a.n_kv_head * p.row_groups,
+                                    a.total_kv_len > 0 ? a.total_kv_len : 0, a.total_kv_len > 0, &s.chunk_len);
+  bool pays;
+  const ScanPlan own = own_scan_plan(a.head_dim, (long long)a.batch * a.n_kv_head * p.row_groups, p.max_kv_seq,
+                                     max_splits_of(a.max_splits), sm_count(), &pays);
+  if (pays) s = own;
+  if (s.needs_workspace()) p.ws_lse = p.ws_o + (size_t)a.batch * a.n_head * s.n_splits * a.head_dim;
+  const int rc = a.head_dim == 128 ? launch_d<128>(p, s, st) : launch_d<64>(p, s, st);
+  if (rc || !a.weights) return rc;
+  const cudaError_t e = launch_overlapped(weight_sums_kernel, dim3((p.max_kv_seq + kSumThreads - 1) / kSumThreads, a.n_kv_head, a.batch),
+                                          dim3(kSumThreads), 0, st, 1, p, a.weights, a.weights_stride[0], a.weights_stride[1]);
+  count_launch();
+  return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
 
 // ---- the typed call with few query rows per KV head

@@ -34,6 +34,7 @@
 #include <vector>
 
 #include "attn_internal.h"
+#include "fast_div.h"
 #include "ptx_sm100.cuh"
 
 namespace tyr {
@@ -61,31 +62,8 @@ constexpr int kExpPolyPairs = 2;           // of every 8 column pairs, computed 
 constexpr int kLaunchRegs = 168, kCtrlRegs = 88, kSoftmaxRegs = 208;
 static_assert(128 * kCtrlRegs + 256 * kSoftmaxRegs <= kThreads * kLaunchRegs, "register pool of the CTA");
 
-// Division of a non-negative 32-bit number by a divisor fixed per launch, as a multiply-high and a
-// shift: q = umulhi(n, mul) >> shr with mul = ceil(2^(31 + ceil(log2 d)) / d), exact for n < 2^31.
-// Every role decodes its item index at every item boundary; the hardware has no integer divider,
-// and seven emulated divisions are about a thousand cycles on the path between two items.
-struct FastDiv {
-  uint32_t mul, shr, d;
-  __device__ __forceinline__ int div(int n) const {
-    return d == 1u ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), mul) >> shr);
-  }
-};
-inline FastDiv make_fastdiv(int d) {
-  FastDiv f;
-  f.d = static_cast<uint32_t>(std::max(d, 1));
-  f.mul = 0;
-  f.shr = 0;
-  if (f.d > 1u) {
-    int lg = 0;
-    while ((1ull << lg) < f.d) ++lg;  // ceil(log2 d)
-    const int pw = 31 + lg;
-    f.mul = static_cast<uint32_t>(((1ull << pw) + f.d - 1) / f.d);
-    f.shr = static_cast<uint32_t>(pw - 32);
-  }
-  return f;
-}
-
+// The item decode divides by multiply-high (fast_div.h): every role decodes its item index at every item boundary, and
+// seven emulated divisions are about a thousand cycles on the path between two items.
 struct PrefillParams {
   __nv_bfloat16* o;
   int64_t o_stride_b, o_stride_h, o_stride_s;

@@ -395,17 +395,223 @@ PyObject* decode_dense(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// x, out, norm_weight, cos, sin, positions, position0, eps, pe, out_at_row0 -> None
+// ---- paged cache
+// a size or count as the C ABI takes it; what does not fit is refused rather than cut off
+int32_t count_of(int64_t v, const char* what) {
+  if (v < INT32_MIN || v > INT32_MAX) throw ValueError(std::string(what) + " does not fit 32 bits");
+  return static_cast<int32_t>(v);
+}
+// a window or a number of first tokens: beyond any length is as good as the greatest length
+int32_t span_of(PyObject* o) {
+  const int64_t v = integer(o);
+  return v > INT32_MAX ? INT32_MAX : v < 0 ? -1 : static_cast<int32_t>(v);
+}
+void same_device(const Tensor& t, const Tensor& as, const char* what) {
+  if (!t.is_cuda() || t.device() != as.device()) throw ValueError(std::string(what) + " must be on the device of the other tensors");
+}
+// int32 [batch], contiguous
+const int32_t* per_sequence(const Tensor& t, const Tensor& as, int64_t batch, const char* what) {
+  same_device(t, as, what);
+  if (t.scalar_type() != at::kInt || t.dim() != 1 || t.size(0) != batch || !t.is_contiguous())
+    throw ValueError(std::string(what) + " must be a contiguous int32 tensor [batch]");
+  return static_cast<const int32_t*>(t.data_ptr());
+}
+void fill_pages(TyrAttnPageTable& p, const Tensor& table, const Tensor& pool, int64_t batch) {
+  same_device(table, pool, "page_table");
+  if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != batch || (table.size(1) > 1 && table.stride(1) != 1))
+    throw ValueError("page_table must be an int32 tensor [batch, max_pages]");
+  p.table = static_cast<const int32_t*>(table.data_ptr());
+  p.table_stride = table.stride(0);
+  p.max_pages = count_of(table.size(1), "page_table");
+  p.n_pages = count_of(pool.size(0), "the number of pages");
+  p.page_size = count_of(pool.size(2), "the page size");
+}
+void require_pool(const Tensor& t, const char* what) {
+  require_cuda(t);
+  if (t.dim() != 4 || t.scalar_type() != at::kBFloat16)
+    throw ValueError(std::string(what) + " must be bf16 [n_pages, n_kv_head, page_size, head_dim]");
+}
+// the pools of K and V and their strides
+void fill_pools(const Tensor& k, const Tensor& v, int64_t* k_stride, int64_t* v_stride) {
+  require_pool(k, "k_pages");
+  require_pool(v, "v_pages");
+  if (v.sizes() != k.sizes()) throw ValueError("k_pages and v_pages differ in shape");
+  same_device(v, k, "v_pages");
+  strides3(k_stride, k);
+  strides3(v_stride, v);
+}
+float* weight_sums(const Tensor& w, const Tensor& as, int64_t batch, int64_t n_kv_head, int64_t* stride) {
+  same_device(w, as, "weights");
+  if (w.scalar_type() != at::kFloat || w.dim() != 3 || w.size(0) != batch || w.size(1) != n_kv_head || (w.size(2) > 1 && w.stride(2) != 1))
+    throw ValueError("weights must be a float32 tensor [batch, n_kv_head, max_kv_seq]");
+  stride[0] = w.stride(0);
+  stride[1] = w.stride(1);
+  return static_cast<float*>(w.data_ptr());
+}
+
+// q, k_pages, v_pages, page_table, kv_lens, max_kv_seq, window_size, n_sink, weights, scale, out, lse, workspace, return_lse,
+// total_kv_len, max_splits -> (out, lse); with `only_bytes` the workspace the call needs
+PyObject* paged_decode_call(PyObject* const* args, Py_ssize_t n, bool only_bytes) {
+  require_count(n, 16);
+  const Tensor &q = tensor(args[0], "q"), &k = tensor(args[1], "k_pages"), &v = tensor(args[2], "v_pages"),
+               &table = tensor(args[3], "page_table"), &lens = tensor(args[4], "kv_lens");
+  const QueryRows r = query_rows(q);
+  if (q.scalar_type() != at::kBFloat16 || (q.dim() == 4 && q.size(2) != 1))
+    throw ValueError("q must be bf16 [batch, n_head, head_dim] or [batch, n_head, 1, head_dim]");
+  TyrAttnPagedDecodeArgs a;
+  std::memset(&a, 0, sizeof(a));
+  fill_pools(k, v, a.k_stride, a.v_stride);
+  same_device(k, q, "k_pages");
+  if (k.size(3) != r.d) throw ValueError("q and the pages differ in head_dim");
+  fill_pages(a.pages, table, k, r.batch);
+  a.kv_lens = per_sequence(lens, q, r.batch, "kv_lens");
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.batch = count_of(r.batch, "the batch");
+  a.n_head = count_of(r.heads, "n_head");
+  a.n_kv_head = count_of(k.size(1), "n_kv_head");
+  a.head_dim = count_of(r.d, "head_dim");
+  const Tensor *w = maybe(args[8], "weights"), *out_in = maybe(args[10], "out"), *lse_in = maybe(args[11], "lse"),
+               *ws_in = maybe(args[12], "workspace");
+  const int64_t cap = (int64_t)a.pages.max_pages * a.pages.page_size;
+  a.max_kv_seq = count_of(args[5] == Py_None ? (w && w->dim() == 3 && w->size(2) < cap ? w->size(2) : cap) : integer(args[5]), "max_kv_seq");
+  a.window_size = span_of(args[6]);
+  a.n_sink = span_of(args[7]);
+  if (w) {
+    a.weights = weight_sums(*w, q, r.batch, k.size(1), a.weights_stride);
+    if (w->size(2) < a.max_kv_seq) throw ValueError("weights holds fewer keys than max_kv_seq");
+  }
+  a.scale = scale_of(args[9]);
+  const bool return_lse = truth(args[13]);
+  const int64_t total = integer(args[14]);
+  a.total_kv_len = total > 0 ? total : 0;
+  a.max_splits = count_of(integer(args[15]), "max_splits");
+  a.q_stride[0] = r.stride_b;
+  a.q_stride[1] = r.stride_h;
+  if (out_in) {
+    require_cuda(*out_in);
+    same_device(*out_in, q, "out");
+    if (out_in->scalar_type() != at::kBFloat16 || out_in->sizes() != q.sizes()) throw ValueError("out must be bf16 and of the shape of q");
+  }
+  if (lse_in) {
+    same_device(*lse_in, q, "lse");
+    if (lse_in->scalar_type() != at::kFloat || !lse_in->is_contiguous() || lse_in->sizes() != q.sizes().slice(0, q.dim() - 1))
+      throw ValueError("lse must be a contiguous float32 tensor [batch, n_head] (with q's fourth axis, [batch, n_head, 1])");
+  }
+  if (only_bytes) {
+    const int64_t need = r.batch == 0 ? 0 : tyr_b200_attn_paged_decode_workspace_bytes(&a);
+    if (need < 0) throw CallError{(int)need};
+    return PyLong_FromLongLong(need);
+  }
+  Tensor out, lse, ws;
+  {
+    NoGil no_gil;
+    c10::cuda::OptionalCUDAGuard guard(q.device());
+    out = out_in ? *out_in : new_tensor(q.sizes(), at::kBFloat16, q.device());
+    if (lse_in) lse = *lse_in;
+    else if (return_lse) lse = new_tensor(q.sizes().slice(0, q.dim() - 1), at::kFloat, q.device());
+    a.o = out.data_ptr();
+    a.o_stride[0] = out.stride(0);
+    a.o_stride[1] = out.stride(1);
+    a.lse = lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr;
+    const int64_t need = r.batch == 0 ? 0 : tyr_b200_attn_paged_decode_workspace_bytes(&a);
+    if (need < 0) throw CallError{(int)need};
+    if (ws_in) {
+      ws = *ws_in;
+      if (ws.scalar_type() != at::kByte || !ws.is_contiguous() || ws.device() != q.device())
+        throw ValueError("workspace must be a contiguous uint8 tensor on q's device");
+    } else if (need > 0) {
+      ws = new_tensor({need}, at::kByte, q.device());
+    }
+    if (ws.defined()) {
+      a.workspace = ws.data_ptr();
+      a.workspace_bytes = ws.numel();
+    }
+    check_rc(tyr_b200_attn_paged_decode(&a, stream_of(q)));
+  }
+  return out_and_lse(out, lse, false);
+}
+PyObject* decode_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&] { return paged_decode_call(args, n, false); });
+}
+PyObject* decode_paged_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&] { return paged_decode_call(args, n, true); });
+}
+
+// k_pages, v_pages, page_table, kv_lens, weights, n_keep, n_recent, n_sink, max_kv_seq, new_lens, kept -> (new_lens, kept)
+PyObject* evict_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    require_count(n, 11);
+    const Tensor &k = tensor(args[0], "k_pages"), &v = tensor(args[1], "v_pages"), &table = tensor(args[2], "page_table"),
+                 &lens = tensor(args[3], "kv_lens"), &w = tensor(args[4], "weights");
+    TyrAttnEvictArgs a;
+    std::memset(&a, 0, sizeof(a));
+    fill_pools(k, v, a.k_stride, a.v_stride);
+    const int64_t batch = lens.dim() == 1 ? lens.size(0) : -1;
+    a.kv_lens = per_sequence(lens, k, batch, "kv_lens");
+    fill_pages(a.pages, table, k, batch);
+    a.weights = weight_sums(w, k, batch, k.size(1), a.weights_stride);
+    a.k = k.data_ptr();
+    a.v = v.data_ptr();
+    a.batch = count_of(batch, "the batch");
+    a.n_kv_head = count_of(k.size(1), "n_kv_head");
+    a.head_dim = count_of(k.size(3), "head_dim");
+    a.n_keep = count_of(integer(args[5]), "n_keep");
+    a.n_recent = count_of(integer(args[6]), "n_recent");
+    a.n_sink = count_of(integer(args[7]), "n_sink");
+    const int64_t cap = (int64_t)a.pages.max_pages * a.pages.page_size;
+    a.max_kv_seq = count_of(args[8] == Py_None ? (w.size(2) < cap ? w.size(2) : cap) : integer(args[8]), "max_kv_seq");
+    if (w.size(2) < a.max_kv_seq) throw ValueError("weights holds fewer keys than max_kv_seq");
+    const Tensor *new_in = maybe(args[9], "new_lens"), *kept_in = maybe(args[10], "kept");
+    if (new_in) per_sequence(*new_in, k, batch, "new_lens");
+    if (kept_in) {
+      same_device(*kept_in, k, "kept");
+      if (kept_in->scalar_type() != at::kInt || !kept_in->is_contiguous() || kept_in->dim() != 3 || kept_in->size(0) != batch ||
+          kept_in->size(1) != k.size(1) || kept_in->size(2) != a.n_keep)
+        throw ValueError("kept must be a contiguous int32 tensor [batch, n_kv_head, n_keep]");
+    }
+    Tensor new_lens, kept;
+    {
+      NoGil no_gil;
+      c10::cuda::OptionalCUDAGuard guard(k.device());
+      new_lens = new_in ? *new_in : new_tensor({batch}, at::kInt, k.device());
+      kept = kept_in ? *kept_in : new_tensor({batch, k.size(1), a.n_keep > 0 ? a.n_keep : 0}, at::kInt, k.device());
+      a.new_lens = static_cast<int32_t*>(new_lens.data_ptr());
+      a.kept = static_cast<int32_t*>(kept.data_ptr());
+      check_rc(tyr_b200_attn_paged_evict(&a, stream_of(k)));
+    }
+    PyObject* t = PyTuple_New(2);
+    if (!t) throw python_error();
+    PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(new_lens)));
+    PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(kept)));
+    return t;
+  });
+}
+
+// x, out, norm_weight, cos, sin, positions, position0, eps, pe, out_at_row0, page_table, rows -> None
 PyObject* qk_prologue(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    require_count(n, 10);
+    require_count(n, 12);
     const Tensor &x = tensor(args[0], "x"), &out = tensor(args[1], "out");
     require_cuda(x);
     require_cuda(out);
     if (x.dim() != 4 || out.dim() != 4 || x.scalar_type() != at::kBFloat16 || out.scalar_type() != at::kBFloat16)
       throw ValueError("x must be bf16 [B,S,H,D] and out bf16 [B,H,cap,D]");
-    const int64_t B = x.size(0), S = x.size(1), H = x.size(2), D = x.size(3), cap = out.size(2);
-    if (out.size(0) != B || out.size(1) != H || out.size(3) != D) throw ValueError("out does not match x");
+    const Tensor *table = maybe(args[10], "page_table"), *rows = maybe(args[11], "rows");
+    const int64_t B = x.size(0), S = x.size(1), H = x.size(2), D = x.size(3);
+    if ((!table && out.size(0) != B) || out.size(1) != H || out.size(3) != D) throw ValueError("out does not match x");
+    TyrAttnPageTable pages;
+    std::memset(&pages, 0, sizeof(pages));
+    if (rows && !table) throw ValueError("rows goes with page_table");
+    if (table) {
+      fill_pages(pages, *table, out, B);
+      same_device(out, x, "out");
+      if (rows) per_sequence(*rows, x, B, "rows");
+      // (dense calls leave the length of positions to the caller)
+      if (args[5] != Py_None) per_sequence(tensor(args[5], "positions"), x, B, "positions");
+    }
+    const int64_t cap = table ? (int64_t)pages.max_pages * pages.page_size : out.size(2);
     const Tensor *w = maybe(args[2], "norm_weight"), *cos = maybe(args[3], "cos"), *sin = maybe(args[4], "sin"),
                  *pos = maybe(args[5], "positions"), *pe = maybe(args[8], "pe");
     for (const Tensor* t : {w, cos, sin, pe})
@@ -423,8 +629,9 @@ PyObject* qk_prologue(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t position0 = integer(args[6]);
     const bool row0 = truth(args[9]);
     if (row0 && S > cap) throw ValueError(std::to_string(S) + " rows do not fit the " + std::to_string(cap) + " rows of out");
+    if (table && row0) throw ValueError("out_at_row0 does not go with page_table");
     if (!pos) {
-      if (position0 < 0 || (!row0 && position0 + S > cap))
+      if (position0 < 0 || (!row0 && !rows && position0 + S > cap))
         throw ValueError("rows " + std::to_string(position0) + ".." + std::to_string(position0 + S - 1) + " do not fit the " +
                          std::to_string(cap) + " rows of out");
       if (max_pos && position0 + S > max_pos)
@@ -453,14 +660,16 @@ PyObject* qk_prologue(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const double eps = PyFloat_AsDouble(args[7]);
     if (eps == -1.0 && PyErr_Occurred()) throw python_error();
     a.eps = static_cast<float>(eps);
-    a.cap = i32(cap);
+    a.cap = table ? 0 : i32(cap);
     a.max_pos = i32(max_pos);
     a.out_at_row0 = row0;
     a.pe_batch_stride = (pe && pe->size(0) > 1) ? pe->stride(0) : 0;
     {
       NoGil no_gil;
       c10::cuda::OptionalCUDAGuard guard(x.device());
-      check_rc(tyr_b200_attn_qk_prologue(&a, stream_of(x)));
+      check_rc(table ? tyr_b200_attn_qk_prologue_paged(&a, &pages, rows ? static_cast<const int32_t*>(rows->data_ptr()) : nullptr,
+                                                       stream_of(x))
+                     : tyr_b200_attn_qk_prologue(&a, stream_of(x)));
     }
     Py_RETURN_NONE;
   });
@@ -474,6 +683,7 @@ PyObject* set_error(PyObject*, PyObject* cls) {
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {FAST(attention_fwd), FAST(attention_bwd), FAST(decode_ragged), FAST(decode_dense), FAST(qk_prologue),
+                           FAST(decode_paged), FAST(decode_paged_workspace), FAST(evict_paged),
                            {"set_error", set_error, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

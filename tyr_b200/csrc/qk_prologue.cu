@@ -13,7 +13,10 @@
 // fp32 with one rounding to bf16 at the end.  HBM-bound: one read and one write per element.
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "attn_internal.h"
+#include "fast_div.h"
 #include "ptx_sm100.cuh"
 
 namespace tyr {
@@ -38,6 +41,15 @@ struct PrologueParams {
   int* status;
 };
 
+// The same into a paged cache: os = {page, head, row}.
+struct PagedPrologueParams : PrologueParams {
+  const int32_t* table;
+  int64_t table_stride;
+  FastDiv by_page;
+  int n_pages;
+  const int32_t* rows;  // cache row of a sequence's first token, or null: its position
+};
+
 __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
   const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
   v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
@@ -50,9 +62,10 @@ __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
 // (they are the same for every head).  A warp covers 512/D consecutive tokens, so for one
 // head its stores are 512/D consecutive rows of the [batch, head, seq, dim] output.
 // kRot: 0 = no rotary, 1 = rotate-half with cos/sin tables, 2 = interleaved pairs with 2x2 tables.
-template <int D, int kRot>
+template <int D, int kRot, class P>
 __global__ void __launch_bounds__(kWarps * 32, kRot == 2 ? 2 : kMinCtasPerSm)
-prologue_kernel(const PrologueParams p) {
+prologue_kernel(const P p) {
+  constexpr bool kPaged = std::is_same<P, PagedPrologueParams>::value;
   constexpr int kHalf = D / 2;
   constexpr int kLanes = D / 16;          // lanes per token
   constexpr int kTokPerWarp = 32 / kLanes;
@@ -69,8 +82,20 @@ prologue_kernel(const PrologueParams p) {
   const int b = (int)(tt / p.seq);
   const int64_t pos = (int64_t)(p.positions ? p.positions[b] : p.position0) + s;  // output row and rotary row
   // a row outside the cache or the rotary table is skipped and reported, never written
-  const int64_t out_row = p.out_at_row0 ? s : pos;
-  const bool in_range = pos >= 0 && out_row < p.cap && (kRot == 0 || pos < p.max_pos);
+  int64_t out_row = p.out_at_row0 ? s : pos;
+  bool in_range = pos >= 0 && out_row < p.cap && (kRot == 0 || pos < p.max_pos);
+  int64_t page = 0;
+  if constexpr (kPaged) {
+    if (p.rows) out_row = (int64_t)p.rows[b] + s;
+    in_range = (pos >= 0 || kRot == 0) && out_row >= 0 && out_row < p.cap && (kRot == 0 || pos < p.max_pos);
+    if (in_range) {
+      const int at = p.by_page.div((int)out_row);
+      page = p.table[b * p.table_stride + at];
+      out_row -= (int64_t)at * p.by_page.d;
+      in_range = page >= 0 && page < p.n_pages;
+      if (!in_range) page = 0;
+    }
+  }
   if (live && !in_range && k8 == 0) atomicOr(p.status, kStatusOutOfRange);
   const bool store = live && in_range;
   const int64_t pos_ld = in_range ? pos : 0;
@@ -94,7 +119,7 @@ prologue_kernel(const PrologueParams p) {
   }
 
   const __nv_bfloat16* xt = p.x + b * p.xs[0] + s * p.xs[1];
-  __nv_bfloat16* ot = p.out + b * p.os[0] + (in_range ? out_row : 0) * p.os[2];
+  __nv_bfloat16* ot = p.out + (kPaged ? page : b) * p.os[0] + (in_range ? out_row : 0) * p.os[2];
 
   const int h_end = min(p.n_head, (int)(blockIdx.y + 1) * p.heads_per_cta);
   for (int h0 = blockIdx.y * p.heads_per_cta; h0 < h_end; h0 += kHeadsInFlight) {
@@ -186,18 +211,19 @@ int heads_per_cta(int n_head, int64_t token_blocks, bool pairs, int64_t group_by
   return h;
 }
 
-template <int D>
-int launch_d(const PrologueParams& p, dim3 grid, cudaStream_t st) {
+template <int D, class P>
+int launch_d(const P& p, dim3 grid, cudaStream_t st) {
   const dim3 block(kWarps * 32);
-  if (p.pe != nullptr) return (int)launch_overlapped(prologue_kernel<D, 2>, grid, block, 0, st, 1, p);
-  if (p.cs != nullptr) return (int)launch_overlapped(prologue_kernel<D, 1>, grid, block, 0, st, 1, p);
-  return (int)launch_overlapped(prologue_kernel<D, 0>, grid, block, 0, st, 1, p);
+  if (p.pe != nullptr) return (int)launch_overlapped(prologue_kernel<D, 2, P>, grid, block, 0, st, 1, p);
+  if (p.cs != nullptr) return (int)launch_overlapped(prologue_kernel<D, 1, P>, grid, block, 0, st, 1, p);
+  return (int)launch_overlapped(prologue_kernel<D, 0, P>, grid, block, 0, st, 1, p);
 }
 
 }  // namespace
 
-int launch_qk_prologue(const TyrAttnPrologueArgs& a, int* status, cudaStream_t st) {
-  PrologueParams p;
+int launch_qk_prologue(const TyrAttnPrologueArgs& a, const TyrAttnPageTable* pages, const int32_t* rows, int* status,
+                       cudaStream_t st) {
+  PagedPrologueParams p;
   p.x = static_cast<const __nv_bfloat16*>(a.x);
   p.out = static_cast<__nv_bfloat16*>(a.out);
   p.w = a.norm_weight;
@@ -219,10 +245,19 @@ int launch_qk_prologue(const TyrAttnPrologueArgs& a, int* status, cudaStream_t s
   p.heads_per_cta = heads_per_cta(a.n_head, blocks, a.pe != nullptr, tokens * a.head_dim * 4 * kHeadsInFlight,
                                   a.cos != nullptr ? (int64_t)a.seq * a.head_dim * 4 : 0);
   const dim3 grid((unsigned)blocks, (a.n_head + p.heads_per_cta - 1) / p.heads_per_cta);
+  if (pages) {
+    p.cap = pages->max_pages * pages->page_size;
+    p.table = pages->table;
+    p.table_stride = pages->table_stride;
+    p.by_page = make_fastdiv(pages->page_size);
+    p.n_pages = pages->n_pages;
+    p.rows = rows;
+  }
+  const PrologueParams& dense = p;
   int rc;
-  if (a.head_dim == 128) rc = launch_d<128>(p, grid, st);
-  else if (a.head_dim == 64) rc = launch_d<64>(p, grid, st);
-  else if (a.head_dim == 256) rc = launch_d<256>(p, grid, st);
+  if (a.head_dim == 128) rc = pages ? launch_d<128>(p, grid, st) : launch_d<128>(dense, grid, st);
+  else if (a.head_dim == 64) rc = pages ? launch_d<64>(p, grid, st) : launch_d<64>(dense, grid, st);
+  else if (a.head_dim == 256) rc = pages ? launch_d<256>(p, grid, st) : launch_d<256>(dense, grid, st);
   else return -TYR_ATTN_ERR_HEAD_DIM;
   if (rc) return rc;
   count_launch();

@@ -284,10 +284,63 @@ def flashDecodeDense(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     return _lib.calls().decode_dense(q, k_cache, v_cache, kv_lens, kv_len, scale, workspace, max_splits)
 
 
+def flashDecodePaged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                     kv_lens: torch.Tensor, max_kv_seq: Optional[int] = None, window_size: int = 0, n_sink: int = 0,
+                     weights: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                     workspace: Optional[torch.Tensor] = None, return_lse: bool = True, total_kv_len: int = 0,
+                     max_splits: int = 64):
+    """One query token per sequence over a KV cache in pages; returns (out, lse).
+
+    q [B, n_head, head_dim] (or [B, n_head, 1, head_dim]) bf16; k_pages, v_pages [n_pages, n_kv_head, page_size,
+    head_dim] bf16, views of any order of those axes with unit stride on the last; page_table int32 [B, max_pages];
+    kv_lens int32 [B], the new token's key included.  Row r of a sequence is row r % page_size of page
+    page_table[b, r // page_size].  `max_kv_seq` (default: all the table can hold) bounds the lengths.  A sequence of
+    length 0 gets zeros and LSE = -inf; a length outside [0, max_kv_seq] is clamped, and it and a used table entry that
+    is no page (NaN rows) set the out-of-range bit of the device status word.
+    `window_size` > 0: only the last `window_size` keys and the first `n_sink` are seen, and read; pages wholly
+    between them may be given back.
+    `weights` float32 [B, n_kv_head, >= max_kv_seq]: the softmax weights each visible key got from the query heads of
+    its group are added in place, the sums `evictPaged` goes by.
+    `total_kv_len`: the sum of the lengths where the host knows it (it steers how the launch is cut).
+    `workspace`: a caller-kept uint8 tensor of `paged_decode_workspace_bytes(...)` bytes, 16-byte aligned, for one call at a
+    time (calls on two streams, or two captured graphs that may run at once, need one each); allocated otherwise.
+    """
+    return _lib.calls().decode_paged(q, k_pages, v_pages, page_table, kv_lens, max_kv_seq, window_size, n_sink, weights, scale,
+                                     out, lse, workspace, return_lse, total_kv_len, max_splits)
+
+
+def paged_decode_workspace_bytes(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                                 kv_lens: torch.Tensor, max_kv_seq: Optional[int] = None, window_size: int = 0, n_sink: int = 0,
+                                 weights: Optional[torch.Tensor] = None, max_splits: int = 64) -> int:
+    """Bytes of `workspace` that `flashDecodePaged` on these tensors would use at most (0: none)."""
+    return _lib.calls().decode_paged_workspace(q, k_pages, v_pages, page_table, kv_lens, max_kv_seq, window_size, n_sink, weights,
+                                               None, None, None, None, False, 0, max_splits)
+
+
+def evictPaged(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
+               weights: torch.Tensor, n_keep: int, n_recent: int, n_sink: int = 0, max_kv_seq: Optional[int] = None,
+               new_lens: Optional[torch.Tensor] = None, kept: Optional[torch.Tensor] = None
+               ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Brings every sequence of a paged cache back to at most `n_keep` keys; returns (new_lens [B], kept [B, n_kv_head, n_keep]).
+
+    Per (sequence, KV head) of more than `n_keep` keys: the first `n_sink`, the last `n_recent`, and of the others those
+    with the greatest `weights` (float32 [B, n_kv_head, >= max_kv_seq], as `flashDecodePaged` sums them; of equal ones the
+    lower position, a NaN below every number) stay.  Their K and V rows move, in the order of their positions, to the
+    sequence's first `n_keep` rows, in place, and their weights likewise; the weights behind them, up to the old
+    length, become 0.  `kept` holds the old positions (-1 behind a sequence's last key), `new_lens` min(length, n_keep);
+    kv_lens itself is not changed and must not be given as new_lens.  Pages behind the new length may be given back.  The
+    sequences may not share pages.
+    """
+    return _lib.calls().evict_paged(k_pages, v_pages, page_table, kv_lens, weights, n_keep, n_recent, n_sink, max_kv_seq, new_lens,
+                                    kept)
+
+
 def qkPrologue(x: torch.Tensor, out: torch.Tensor, norm_weight: Optional[torch.Tensor] = None,
                cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
                positions: Optional[torch.Tensor] = None, position0: int = 0, eps: float = 1e-6,
-               pe: Optional[torch.Tensor] = None, out_at_row0: bool = False):
+               pe: Optional[torch.Tensor] = None, out_at_row0: bool = False,
+               page_table: Optional[torch.Tensor] = None, rows: Optional[torch.Tensor] = None):
     """Fused per-head RMSNorm + rotary embedding + [B,S,H,D] -> [B,H,S,D] layout change,
     written into `out` [B,H,cap,D] at rows positions[b] + s (in place: a KV-cache append
     when `out` is the cache).  One pass instead of applyHeadNorm
@@ -303,8 +356,13 @@ def qkPrologue(x: torch.Tensor, out: torch.Tensor, norm_weight: Optional[torch.T
     Rows that would fall outside `out` or outside the rotary table are refused here when the
     position is known on the host (position0); with device-side `positions` the kernel skips
     them and sets the out-of-range bit of the device status word.
+    `page_table` (int32 [B, max_pages]) makes `out` the pool of a paged cache, [n_pages, H, page_size, D]: token s of
+    sequence b goes to cache row positions[b] + s, which is row r % page_size of page page_table[b, r // page_size].
+    `rows` (int32 [B]) gives the first of those cache rows where it is not the rotary position: a cache that
+    keys were evicted from (`evictPaged`) is shorter than the text.  A row outside the table, or whose entry
+    is no page of the pool, is skipped and sets the same status bit.
     """
-    _lib.calls().qk_prologue(x, out, norm_weight, cos, sin, positions, position0, eps, pe, out_at_row0)
+    _lib.calls().qk_prologue(x, out, norm_weight, cos, sin, positions, position0, eps, pe, out_at_row0, page_table, rows)
     return out
 
 
