@@ -115,6 +115,14 @@ int tyr_b200_attn_prefill(const TyrAttnPrefillArgs* args, void* stream);
  * uncut or in clusters), negative TYR_ATTN_ERR_* on bad arguments. */
 int64_t tyr_b200_attn_prefill_workspace_bytes(const TyrAttnPrefillArgs* args);
 
+/* The windowed call with `n_sink` first tokens that stay visible: key j is visible to query i when
+ * j <= i and (i - j < window_size or j < n_sink).  No counterpart in the reference; beside
+ * lean_torch_sdpa_gqa_window for models whose windowed layers keep the first tokens in sight.
+ * The other arguments are those of tyr_b200_attn_prefill (check_mode too) and n_sink = 0 is that call.
+ * n_sink > 0 needs window_size > 0 and no key_mask (-TYR_ATTN_ERR_SHAPE otherwise; a negative n_sink too):
+ * every query sees its own key, so no row is empty.  One launch, no workspace. */
+int tyr_b200_attn_prefill_sinks(const TyrAttnPrefillArgs* args, int32_t n_sink, void* stream);
+
 /* Contiguous-layout forms whose argument lists mirror the Lean externs one to
  * one: tensor handles become device pointers, the result tensor becomes the
  * caller-allocated `out`, and the stream is explicit.  bf16 only.
@@ -426,6 +434,13 @@ typedef struct TyrAttnBackwardArgs {
  * zero) dQ has no element and dK, dV are written as zeros; without keys dQ is written as zeros. */
 uint64_t tyr_b200_attn_backward_workspace_bytes(int32_t batch, int32_t n_head, int32_t q_seq);
 int tyr_b200_attn_backward(const TyrAttnBackwardArgs* args, void* stream);
+
+/* Gradients of tyr_b200_attn_prefill_sinks, with its rules for n_sink; n_sink = 0 is the call above.  The first keys are
+ * seen by every query, so where that would leave them to few SMs their query rows are shared out and the partial
+ * sums, in the workspace, added in a fixed order by a fourth launch.  workspace: 16-byte aligned, of the size the
+ * function says (at least that of the call above; negative TYR_ATTN_ERR_* on bad arguments). */
+int64_t tyr_b200_attn_backward_sinks_workspace_bytes(const TyrAttnBackwardArgs* args, int32_t n_sink);
+int tyr_b200_attn_backward_sinks(const TyrAttnBackwardArgs* args, int32_t n_sink, void* stream);
 
 /* ------------------------------------------------------------------------
  * Host-buffer call: same arithmetic as tyr_b200_attn_prefill, but every

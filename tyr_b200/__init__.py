@@ -7,8 +7,9 @@ include/tyr_b200_attn.h.  PyTorch is used for device memory and streams only.
 from . import nn  # noqa: F401
 from .nn import (attentionFwd, evictPaged, flashDecode, flashDecodePaged, scaled_dot_product_attention,  # noqa: F401
                  scaledDotProductAttentionGQA, scaledDotProductAttentionGQAQKV,
-                 scaledDotProductAttentionGQAMask, scaledDotProductAttentionGQAWindow)
+                 scaledDotProductAttentionGQAMask, scaledDotProductAttentionGQAWindow,
+                 scaledDotProductAttentionGQAWindowSinks)
 
 __all__ = ["nn", "attentionFwd", "evictPaged", "flashDecode", "flashDecodePaged", "scaled_dot_product_attention",
            "scaledDotProductAttentionGQA", "scaledDotProductAttentionGQAQKV",
-           "scaledDotProductAttentionGQAWindow", "scaledDotProductAttentionGQAMask"]
+           "scaledDotProductAttentionGQAWindow", "scaledDotProductAttentionGQAWindowSinks", "scaledDotProductAttentionGQAMask"]

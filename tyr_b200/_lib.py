@@ -20,12 +20,13 @@ DECODE_STATIC_SCRATCH_BYTES = 16 << 20   # TYR_ATTN_DECODE_STATIC_SCRATCH_BYTES
 
 # every symbol include/tyr_b200_attn.h declares
 EXPORTS = [
-    "tyr_b200_attn_prefill", "tyr_b200_attn_prefill_workspace_bytes", "tyr_b200_sdpa_4d", "tyr_b200_sdpa_gqa", "tyr_b200_sdpa_gqa_qkv",
+    "tyr_b200_attn_prefill", "tyr_b200_attn_prefill_sinks", "tyr_b200_attn_prefill_workspace_bytes", "tyr_b200_sdpa_4d", "tyr_b200_sdpa_gqa", "tyr_b200_sdpa_gqa_qkv",
     "tyr_b200_sdpa_gqa_window", "tyr_b200_sdpa_gqa_mask",
     "tyr_b200_attn_decode_workspace_bytes", "tyr_b200_attn_decode", "tyr_b200_attn_decode_static",
     "tyr_b200_attn_paged_decode_workspace_bytes", "tyr_b200_attn_paged_decode", "tyr_b200_attn_paged_evict",
     "tyr_b200_attn_merge", "tyr_b200_attn_qk_prologue", "tyr_b200_attn_qk_prologue_paged",
     "tyr_b200_attn_backward_workspace_bytes", "tyr_b200_attn_backward",
+    "tyr_b200_attn_backward_sinks_workspace_bytes", "tyr_b200_attn_backward_sinks",
     "tyr_b200_attn_prefill_host", "tyr_b200_attn_device_status", "tyr_b200_attn_device_check",
     "tyr_b200_attn_test_set_wait_limit", "tyr_b200_attn_test_stalled_wait", "tyr_b200_attn_strerror",
     "tyr_b200_attn_abi_version", "tyr_b200_attn_launch_count",
@@ -120,6 +121,12 @@ def load() -> ctypes.CDLL:
     L = ctypes.CDLL(LIB_PATH)
     L.tyr_b200_attn_prefill.argtypes = [ctypes.POINTER(PrefillArgs), vp]
     L.tyr_b200_attn_prefill.restype = ctypes.c_int
+    L.tyr_b200_attn_prefill_sinks.argtypes = [ctypes.POINTER(PrefillArgs), c_i32, vp]
+    L.tyr_b200_attn_prefill_sinks.restype = ctypes.c_int
+    L.tyr_b200_attn_backward_sinks_workspace_bytes.argtypes = [ctypes.POINTER(BackwardArgs), c_i32]
+    L.tyr_b200_attn_backward_sinks_workspace_bytes.restype = c_i64
+    L.tyr_b200_attn_backward_sinks.argtypes = [ctypes.POINTER(BackwardArgs), c_i32, vp]
+    L.tyr_b200_attn_backward_sinks.restype = ctypes.c_int
     L.tyr_b200_attn_prefill_host.argtypes = [ctypes.POINTER(PrefillArgs), c_i32]
     L.tyr_b200_attn_prefill_host.restype = ctypes.c_int
     L.tyr_b200_sdpa_4d.argtypes = [c_u64] * 4 + [vp] * 4 + [c_f64, c_u8, vp]

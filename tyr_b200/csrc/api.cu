@@ -129,6 +129,13 @@ int check_prefill(const TyrAttnPrefillArgs* a) {
   return 0;
 }
 
+// First tokens beside a window.  A window beyond the keys is taken as all of them.
+int check_sinks(int n_sink, int kv_seq, const void* key_mask, int32_t* window) {
+  if (n_sink < 0 || (n_sink > 0 && (*window <= 0 || key_mask))) return -TYR_ATTN_ERR_SHAPE;
+  if (n_sink > 0 && kv_seq > 0) *window = std::min(*window, kv_seq);
+  return 0;
+}
+
 // ---- paged cache
 int check_page_table(const TyrAttnPageTable& t, int64_t max_kv_seq) {
   if (t.max_pages <= 0 || t.n_pages <= 0 || t.page_size <= 0 || t.table_stride < 0) return -TYR_ATTN_ERR_SHAPE;
@@ -217,19 +224,28 @@ using namespace tyr;
 
 extern "C" {
 
-int tyr_b200_attn_prefill(const TyrAttnPrefillArgs* a, void* stream) {
+static int prefill(const TyrAttnPrefillArgs* a, int n_sink, void* stream) {
   if (const int kind = empty_kind(a)) return kind == 1 ? 0 : launch_no_keys(*a, static_cast<cudaStream_t>(stream));
   int rc = check_prefill(a);
   if (rc) return rc;
   const float scale = resolve_scale(a->scale, a->head_dim);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->check_mode) return launch_prefill_check(*a, scale, st);
+  if (a->check_mode) return launch_prefill_check(*a, n_sink, scale, st);
   int dev = 0;
   if ((rc = current_device_checked(&dev))) return rc;
   DeviceState* ds = device_state(dev);
   if (!ds) return -TYR_ATTN_ERR_NO_DEVICE;
   if (few_rows_call(*a)) return launch_few_rows(*a, scale, ds->status, st);
-  return launch_prefill_sm100(*a, scale, ds->status, st);
+  return launch_prefill_sm100(*a, n_sink, scale, ds->status, st);
+}
+
+int tyr_b200_attn_prefill(const TyrAttnPrefillArgs* a, void* stream) { return prefill(a, 0, stream); }
+
+int tyr_b200_attn_prefill_sinks(const TyrAttnPrefillArgs* a, int32_t n_sink, void* stream) {
+  if (!a) return -TYR_ATTN_ERR_NULL;
+  TyrAttnPrefillArgs d = *a;
+  const int rc = check_sinks(n_sink, a->kv_seq, a->key_mask, &d.window_size);
+  return rc ? rc : prefill(&d, n_sink, stream);
 }
 
 int tyr_b200_sdpa_4d(uint64_t batch, uint64_t n_head, uint64_t seq, uint64_t head_dim, const void* q,
@@ -405,7 +421,7 @@ uint64_t tyr_b200_attn_backward_workspace_bytes(int32_t batch, int32_t n_head, i
   return backward_workspace_bytes(batch, n_head, q_seq);
 }
 
-int tyr_b200_attn_backward(const TyrAttnBackwardArgs* a, void* stream) {
+static int backward(const TyrAttnBackwardArgs* a, int n_sink, void* stream) {
   // Zero extents as autograd of ATen's operator treats them: without queries (or heads, or a batch)
   // dQ has no element and dK, dV are zeros; without keys dK, dV have no element and dQ is zeros.
   if (a && a->batch >= 0 && a->n_head >= 0 && a->n_kv_head >= 0 && a->q_seq >= 0 && a->kv_seq >= 0 &&
@@ -445,14 +461,36 @@ int tyr_b200_attn_backward(const TyrAttnBackwardArgs* a, void* stream) {
       if (dims[i] > 1 && (strides[t][i] <= 0 || (strides[t][i] & 7))) return -TYR_ATTN_ERR_ALIGN;
   }
   if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 15u) ||
-      a->workspace_bytes < backward_workspace_bytes(a->batch, a->n_head, a->q_seq))
+      a->workspace_bytes < (n_sink > 0 ? backward_sinks_workspace_bytes(*a, n_sink)
+                                       : backward_workspace_bytes(a->batch, a->n_head, a->q_seq)))
     return -TYR_ATTN_ERR_WORKSPACE;
   int dev = 0, rc;
   if ((rc = current_device_checked(&dev))) return rc;
   DeviceState* ds = device_state(dev);
   if (!ds) return -TYR_ATTN_ERR_NO_DEVICE;
-  return launch_backward_sm100(*a, resolve_scale(a->scale, a->head_dim), ds->status,
+  return launch_backward_sm100(*a, n_sink, resolve_scale(a->scale, a->head_dim), ds->status,
                                static_cast<cudaStream_t>(stream));
+}
+
+int tyr_b200_attn_backward(const TyrAttnBackwardArgs* a, void* stream) { return backward(a, 0, stream); }
+
+int tyr_b200_attn_backward_sinks(const TyrAttnBackwardArgs* a, int32_t n_sink, void* stream) {
+  if (!a) return -TYR_ATTN_ERR_NULL;
+  TyrAttnBackwardArgs d = *a;
+  const int rc = check_sinks(n_sink, a->kv_seq, a->key_mask, &d.window_size);
+  return rc ? rc : backward(&d, n_sink, stream);
+}
+
+int64_t tyr_b200_attn_backward_sinks_workspace_bytes(const TyrAttnBackwardArgs* a, int32_t n_sink) {
+  if (!a) return -TYR_ATTN_ERR_NULL;
+  TyrAttnBackwardArgs d = *a;
+  const int rc = check_sinks(n_sink, a->kv_seq, a->key_mask, &d.window_size);
+  if (rc) return rc;
+  if (a->batch < 0 || a->n_head < 0 || a->n_kv_head < 0 || a->q_seq < 0 || a->kv_seq < 0) return -TYR_ATTN_ERR_SHAPE;
+  if (a->batch == 0 || a->n_head == 0 || a->n_kv_head == 0 || a->q_seq == 0 || a->kv_seq == 0) return 0;
+  if (a->n_head % a->n_kv_head != 0) return -TYR_ATTN_ERR_SHAPE;
+  if (a->head_dim != 64 && a->head_dim != 128) return -TYR_ATTN_ERR_HEAD_DIM;
+  return (int64_t)(n_sink > 0 ? backward_sinks_workspace_bytes(d, n_sink) : backward_workspace_bytes(a->batch, a->n_head, a->q_seq));
 }
 
 int64_t tyr_b200_attn_prefill_workspace_bytes(const TyrAttnPrefillArgs* a) {

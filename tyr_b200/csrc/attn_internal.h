@@ -66,16 +66,18 @@ long long wait_limit_cycles();
 int launch_stalled_wait(long long limit_cycles, int* status, cudaStream_t st);
 
 // prefill_sm100.cu — tcgen05/TMA kernel, bf16, head_dim in {64,128}.
-int launch_prefill_sm100(const TyrAttnPrefillArgs& a, float scale, int* status, cudaStream_t st);
+// n_sink: first tokens that stay visible beside the window (0: none).
+int launch_prefill_sm100(const TyrAttnPrefillArgs& a, int n_sink, float scale, int* status, cudaStream_t st);
 long long prefill_split_workspace_bytes(const TyrAttnPrefillArgs& a);  // 0: the launch would not split
 // 128-byte-swizzled 64 x 128 box map over a bf16 [batch, heads, seq, d] tensor with element strides
 // {batch, head, seq}; encoded maps are cached per thread (prefill_sm100.cu).
 int make_tile_map(CUtensorMap* m, const void* ptr, int batch, int heads, int seq, int d, const int64_t* stride);
 // backward_sm100.cu — tcgen05/TMA kernels, bf16, head_dim in {64,128}.
 size_t backward_workspace_bytes(int batch, int n_head, int q_seq);
-int launch_backward_sm100(const TyrAttnBackwardArgs& a, float scale, int* status, cudaStream_t st);
+size_t backward_sinks_workspace_bytes(const TyrAttnBackwardArgs& a, int n_sink);
+int launch_backward_sm100(const TyrAttnBackwardArgs& a, int n_sink, float scale, int* status, cudaStream_t st);
 // check_fp32.cu — fp32-FMA kernel, bf16 or fp32 I/O, any head_dim <= 256.
-int launch_prefill_check(const TyrAttnPrefillArgs& a, float scale, cudaStream_t st);
+int launch_prefill_check(const TyrAttnPrefillArgs& a, int n_sink, float scale, cudaStream_t st);
 // decode_splitkv.cu
 size_t decode_workspace_bytes(int batch, int n_head, int head_dim, int max_kv_seq, int max_splits);
 int decode_num_splits(int max_kv_seq, int max_splits, int* chunk_len);

@@ -118,6 +118,10 @@ struct BwdParams {
   long long wait_limit;  // cycles any single barrier wait may take before the CTA gives up
   int parts;             // dK/dV kernel: CTAs of a cluster that share a unit (1: none)
   int wait_first;        // dQ kernel: dQ overlaps an input, so the dK/dV kernel has to be through
+  // kSink only: the first n_sink keys are visible to every later row beside the window.  Their sink_blk key blocks are
+  // done in sink_parts units each, whose partial dK and dV (fp32) go to sink_out and are added by bwd_sink_merge_kernel.
+  int n_sink, sink_blk, sink_parts;
+  float* sink_out;       // [sink_blk][sink_parts][batch][n_kv_head][dK, dV][128 keys][D]; null when sink_parts is 1
 };
 
 constexpr uint32_t kBwdDescHi = umma_desc_hi(1024);
@@ -174,19 +178,37 @@ struct KvUnit {
   int lo;        // first query block with a row >= the unit's first key
   int per_head;  // query blocks streamed per query head
   int n_iter;    // per_head * group; 0 when no query sees these keys
+  int first;     // kSink: the unit's first streamed pair of the block's, and which of its parts it is
+  int part;
 };
+template <bool kSink>
+__device__ __forceinline__ int kv_units(const BwdParams& p) {
+  return (p.n_kblk + (kSink ? p.sink_blk * (p.sink_parts - 1) : 0)) * p.n_kv_head * p.batch;
+}
+template <bool kSink>
 __device__ __forceinline__ KvUnit kv_unit(int u, const BwdParams& p) {
   KvUnit w;
+  w.first = w.part = 0;
   const int lvl = u / (p.n_kv_head * p.batch);
   const int rem = u - lvl * p.n_kv_head * p.batch;
   w.head = rem % p.n_kv_head;
   w.b = rem / p.n_kv_head;
   w.blk = lvl;
+  const int in_parts = kSink ? p.sink_blk * p.sink_parts : 0;  // units per head of the blocks of first tokens
+  if (kSink) {
+    w.blk = lvl < in_parts ? lvl / p.sink_parts : lvl - in_parts + p.sink_blk;
+    w.part = lvl < in_parts ? lvl % p.sink_parts : 0;
+  }
   w.lo = p.causal ? min(w.blk, p.n_qblk) : 0;
   int hi = p.n_qblk;  // one past the last query block that sees a key of the unit
-  if (p.window > 0) hi = min(hi, (w.blk * kT + kT - 1 + p.window - 1) / kT + 1);
+  if (p.window > 0 && !(kSink && w.blk < p.sink_blk)) hi = min(hi, (w.blk * kT + kT - 1 + p.window - 1) / kT + 1);
   w.per_head = max(hi - w.lo, 0);
   w.n_iter = w.per_head * p.group;
+  if (kSink && lvl < in_parts) {
+    const int n = w.n_iter;
+    w.first = (int)((long long)n * w.part / p.sink_parts);
+    w.n_iter = (int)((long long)n * (w.part + 1) / p.sink_parts) - w.first;
+  }
   return w;
 }
 
@@ -203,7 +225,8 @@ struct UnitPart {
 // tiles of the unit stay in shared memory (the next unit's are fetched as soon as the unit's last
 // score products have read them), Q and dO stream.  Barrier phases run on across units: every role
 // counts streamed tile pairs (`it`) and units with work (`rc`) for itself.
-template <int D, bool kCluster>
+// kSink: first tokens that stay visible beside a window (BwdParams).
+template <int D, bool kCluster, bool kSink>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                 const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
@@ -218,12 +241,12 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   const uint32_t sBar = base + C::kBarOff;
   auto bar = [&](int i) { return sBar + 8u * i; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_units = p.n_kblk * p.n_kv_head * p.batch;
+  const int n_units = kv_units<kSink>(p);
   const int n_rounds = kCluster ? 1 : rounds_of(n_units);
   const UnitPart part = {kCluster ? static_cast<int>(cluster_rank()) : 0, kCluster ? p.parts : 1};
   auto unit_at = [&](int round) { return kCluster ? static_cast<int>(blockIdx.x) / part.size : unit_of_round(round, n_units); };
   auto unit = [&](int u) {
-    KvUnit w = kv_unit(u, p);
+    KvUnit w = kv_unit<kSink>(u, p);
     if (kCluster) w.n_iter = part.pairs(w.n_iter);
     return w;
   };
@@ -282,7 +305,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
           const int s = it % C::kStages;
           if (it >= C::kStages) ok = mbar_wait_q(bar(C::str_empty + s), ((it / C::kStages) - 1) & 1, abortp);
           if (!ok) break;
-          const int gi = kCluster ? part.pair(i) : i;
+          const int gi = kCluster ? part.pair(i) : kSink ? w.first + i : i;
           const int hq = w.head * p.group + gi / w.per_head, qblk = w.lo + gi % w.per_head;
           const uint32_t dst = base + C::kStr + s * 2 * C::kTileBytes;
           mbar_expect_tx(bar(C::str_full + s), 2 * C::kTileBytes + C::kStatBytes);
@@ -425,11 +448,12 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const int col0 = (w.lo + (kCluster ? part.pair(i) : i) % w.per_head) * kT;  // first query of the score columns
+        // first query of the score columns
+        const int col0 = (w.lo + (kCluster ? part.pair(i) : kSink ? w.first + i : i) % w.per_head) * kT;
         // under the causal mask a key row keeps the query columns with query >= key
         int c_first = p.causal ? row0 + r - col0 : 0;
         // sliding window: the key also drops out for queries with query - key >= window
-        const int c_limit = p.window > 0 ? row0 + r - col0 + p.window : kT;
+        const int c_limit = p.window > 0 && !(kSink && row0 + r < p.n_sink) ? row0 + r - col0 + p.window : kT;
         // a padding key sees no query at all
         if (p.key_mask != nullptr && (row0 + r >= p.kv_seq || p.key_mask[w.b * p.key_mask_stride + row0 + r] == 0))
           c_first = kT;
@@ -565,6 +589,28 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       }
       const int row = row0 + r;
       const bool row_ok = row < p.kv_seq;
+      if (kSink && w.blk < p.sink_blk && p.sink_parts > 1) {
+        float* out = p.sink_out + ((((int64_t)w.blk * p.sink_parts + w.part) * p.batch + w.b) * p.n_kv_head + w.head) * (2 * kT * D);
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+          for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
+            uint32_t o[32];
+            tmem_ld32(tmem + lane_addr + (which ? C::kTmemAcc2 : C::kTmemAcc1) + c * 32, o);
+            tmem_wait_ld();
+            tmem_ld_ready(o);
+            float4* to = reinterpret_cast<float4*>(out + (which * kT + r) * D + c * 32);
+#pragma unroll
+            for (int q4 = 0; q4 < 8; ++q4)
+              to[q4] = make_float4(__uint_as_float(o[q4 * 4]), __uint_as_float(o[q4 * 4 + 1]), __uint_as_float(o[q4 * 4 + 2]),
+                                   __uint_as_float(o[q4 * 4 + 3]));
+          }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::acc_free));
+        ++rc;
+        continue;
+      }
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         const uint32_t tA = tmem + lane_addr + (which ? C::kTmemAcc2 : C::kTmemAcc1);
@@ -608,7 +654,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     // Every CTA sums its share of the rows over the cluster.  All threads come here, also after a wait
     // that gave up (the sums are then as useless as the status says).
     cluster_sync();
-    const KvUnit w = kv_unit(unit_at(0), p);
+    const KvUnit w = kv_unit<kSink>(unit_at(0), p);
     const int rows = kT / part.size, row0 = part.rank * rows;
     const uint32_t buf = base + C::kStr;
     // a group of 32 elements: 8 neighbouring column quadruples of 4 rows
@@ -693,6 +739,7 @@ struct QUnit {
   int lo;      // first key block a row of the unit sees (> 0 only under a sliding window)
   int n_iter;  // key blocks lo .. lo + n_iter - 1
 };
+template <bool kSink>
 __device__ __forceinline__ QUnit q_unit(int u, const BwdParams& p) {
   QUnit w;
   const int lvl = u / (p.n_head * p.batch);
@@ -701,11 +748,18 @@ __device__ __forceinline__ QUnit q_unit(int u, const BwdParams& p) {
   w.b = rem / p.n_head;
   w.blk = p.n_qblk - 1 - lvl;
   w.lo = p.window > 0 ? max(w.blk * kT - p.window + 1, 0) / kT : 0;
+  if (kSink) w.lo = max(w.lo - p.sink_blk, 0);  // blocks no row sees, behind those of the first tokens
   w.n_iter = (p.causal ? min(p.n_kblk, w.blk + 1) : p.n_kblk) - w.lo;
   return w;
 }
 
-template <int D>
+// the i-th key block a unit visits: those of the first tokens, then those of the window
+template <bool kSink>
+__device__ __forceinline__ int key_block(int lo, int i, int sink_blk) {
+  return kSink && i < sink_blk ? i : lo + i;
+}
+
+template <int D, bool kSink>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
               const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -757,7 +811,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       for (int round = 0; round < rounds_of(n_units) && ok; ++round, ++rc) {
         const int u = unit_of_round(round, n_units);
         if (u < 0) break;  // only the last round can be short
-        const QUnit w = q_unit(u, p);
+        const QUnit w = q_unit<kSink>(u, p);
         const int hkv = w.head / p.group;
         if (rc > 0) ok = mbar_wait_q(bar(C::res_empty), (rc - 1) & 1, abortp);
         if (!ok) break;
@@ -775,14 +829,14 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
 #pragma unroll
           for (int kb = 0; kb < C::kBoxes; ++kb)
             tma_load_4d(base + C::kK + ks * C::kTileBytes + kb * C::kBoxBytes, &tm_k, bar(C::k_full + ks), kb * 64,
-                        (w.lo + i) * kT, hkv, w.b);
+                        key_block<kSink>(w.lo, i, p.sink_blk) * kT, hkv, w.b);
           if (it >= C::kVStages) ok = mbar_wait_q(bar(C::v_empty + vs), ((it / C::kVStages) - 1) & 1, abortp);
           if (!ok) break;
           mbar_expect_tx(bar(C::v_full + vs), C::kTileBytes);
 #pragma unroll
           for (int kb = 0; kb < C::kBoxes; ++kb)
             tma_load_4d(base + C::kV + vs * C::kTileBytes + kb * C::kBoxBytes, &tm_v, bar(C::v_full + vs), kb * 64,
-                        (w.lo + i) * kT, hkv, w.b);
+                        key_block<kSink>(w.lo, i, p.sink_blk) * kT, hkv, w.b);
         }
       }
     }
@@ -809,7 +863,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       for (int round = 0; round < rounds_of(n_units) && ok; ++round, ++rc) {
         const int u = unit_of_round(round, n_units);
         if (u < 0) break;  // only the last round can be short
-        const QUnit w = q_unit(u, p);
+        const QUnit w = q_unit<kSink>(u, p);
         ok = mbar_wait_q(bar(C::res_full), rc & 1, abortp);
         // S and dP of the previous unit's last pair must be in the elementwise warps' registers
         if (ok && it > 0) ok = mbar_wait_q(bar(C::sdp_free), (it - 1) & 1, abortp);
@@ -849,7 +903,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     for (int round = 0; round < rounds_of(n_units) && ok; ++round, ++rc) {
       const int u = unit_of_round(round, n_units);
       if (u < 0) break;  // only the last round can be short
-      const QUnit w = q_unit(u, p);
+      const QUnit w = q_unit<kSink>(u, p);
       const int row0 = w.blk * kT;
       const int64_t at = ((int64_t)w.b * p.n_head + w.head) * p.sq_pad + row0 + r;
       const float nl_row = ld_gpu_f32(p.neg_lse2 + at), nd_row = ld_gpu_f32(p.neg_delta_s + at);
@@ -876,10 +930,11 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         if (lane == 0) mbar_arrive(bar(C::sdp_free));
 
         // keys this query row keeps under the causal mask: key <= query
-        const int col0 = (w.lo + i) * kT;  // first key of the score columns
+        const int col0 = key_block<kSink>(w.lo, i, p.sink_blk) * kT;  // first key of the score columns
         const int c_limit = p.causal ? row0 + r - col0 + 1 : kT;
         // sliding window: keys with query - key >= window drop out
         const int c_first = p.window > 0 ? row0 + r - p.window + 1 - col0 : 0;
+        const int c_shown = kSink ? p.n_sink - col0 : 0;  // first tokens
         // padding keys: lane l fetches the mask bytes of keys 2l, 2l+1 of this warp's 64 columns, two
         // ballots spread them to every row; column j of the 64 is bit (j >> 1) of ballot (j & 1)
         uint32_t vb[2] = {0xffffffffu, 0xffffffffu};
@@ -901,7 +956,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           if (masked) {
 #pragma unroll
             for (int x = 0; x < 32; ++x)
-              if (c * 32 + x >= c_limit || c * 32 + x < c_first || !((vb[x & 1] >> ((32 * step + x) >> 1)) & 1u))
+              if (c * 32 + x >= c_limit || (c * 32 + x < c_first && (!kSink || c * 32 + x >= c_shown)) || !((vb[x & 1] >> ((32 * step + x) >> 1)) & 1u))
                 sr[x] = 0xff800000u;  // -inf: P = 0
           }
           uint32_t pk_s[16];
@@ -977,6 +1032,34 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   grid_dependency_wait();  // this grid is complete only when the dK/dV kernel is: what follows sees all three gradients
 }
 
+// dK and dV of the first tokens' key blocks: the sum of their parts, in order.  Four columns of a row per thread.
+template <int D>
+__global__ void __launch_bounds__(256) bwd_sink_merge_kernel(const BwdParams p) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t heads = (int64_t)p.batch * p.n_kv_head, per_head = 2 * kT * (D / 4);
+  if (i >= p.sink_blk * heads * per_head) return;
+  const int64_t bh = i / per_head % heads;
+  const int blk = (int)(i / per_head / heads), e = (int)(i % per_head);
+  const int which = e / (kT * (D / 4)), r = e / (D / 4) % kT, col = e % (D / 4) * 4;
+  const int row = blk * kT + r;
+  if (row >= p.kv_seq) return;
+  const float* from = p.sink_out + (blk * p.sink_parts * heads + bh) * (2 * kT * D) + (which * kT + r) * D + col;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = 0; k < p.sink_parts; ++k) {
+    const float4 v = *reinterpret_cast<const float4*>(from + k * heads * (2 * kT * D));
+    acc.x += v.x;
+    acc.y += v.y;
+    acc.z += v.z;
+    acc.w += v.w;
+  }
+  const int64_t* st = which ? p.out2_stride : p.out1_stride;
+  __nv_bfloat16* to = (which ? p.out2 : p.out1) + bh / p.n_kv_head * st[0] + bh % p.n_kv_head * st[1] + row * st[2] + col;
+  *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+}
+
 // Row statistics of the backward: one group of D/8 lanes per query row, 16-byte loads.
 // (The pointers are not __restrict__: its CTAs are resident while the grid before may still be writing O, dO and the
 // LSE, which rules the read-only path out.)
@@ -1020,7 +1103,7 @@ bwd_rowstats_kernel(const __nv_bfloat16* o, const __nv_bfloat16* d_o, const floa
 
 // CTAs that share a unit of the dK/dV kernel (unit_parts.h).  How many clusters run at once depends on how the SMs are
 // spread over the GPCs: asked for once per device.
-template <int D>
+template <int D, bool kSink>
 int unit_parts(const BwdParams& p, int dev, int sms) {
   static std::atomic<int> known[64][kPartsChoices] = {};  // per device; 0: not asked yet, else capacity + 1
   if ((long long)p.n_kblk * p.n_kv_head * p.batch >= 2ll * sms || p.q_seq >= kOneOrderSeq || p.kv_seq >= kOneOrderSeq) return 1;
@@ -1039,7 +1122,7 @@ int unit_parts(const BwdParams& p, int dev, int sms) {
       cfg.attrs = &attr;
       cfg.numAttrs = 1;
       int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, bwd_dkdv_kernel<D, true>, &cfg) != cudaSuccess) {
+      if (cudaOccupancyMaxActiveClusters(&n, bwd_dkdv_kernel<D, true, kSink>, &cfg) != cudaSuccess) {
         cudaGetLastError();  // no clusters of this size then
         n = 0;
       }
@@ -1056,11 +1139,37 @@ int unit_parts(const BwdParams& p, int dev, int sms) {
   z.group = p.group;
   z.window = p.window;
   z.causal = p.causal != 0;
+  z.sink_blk = kSink ? p.sink_blk : 0;
   return choose_unit_parts(z, sms, capacity);
 }
 
-template <int D>
-int launch_bwd(const TyrAttnBackwardArgs& a, float scale, int* status, cudaStream_t st) {
+int sms_of_device() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
+    sms = 148;
+  return sms;
+}
+
+// The first tokens' key blocks, and in how many units each of them is done where a unit is one CTA's
+struct SinkPlan {
+  int blk, parts;
+  size_t bytes;  // of the parts' partial sums
+};
+SinkPlan sink_plan(const TyrAttnBackwardArgs& a, int n_sink, int sms) {
+  SinkPlan s{0, 1, 0};
+  if (n_sink <= 0) return s;
+  const int n_kblk = (a.kv_seq + kT - 1) / kT, n_qblk = (a.q_seq + kT - 1) / kT;
+  s.blk = (std::min(n_sink, a.kv_seq) + kT - 1) / kT;
+  s.parts = choose_sink_parts(n_kblk, n_qblk, a.n_kv_head, a.n_head / a.n_kv_head, a.window_size, s.blk, sms);
+  if (s.parts > 1) s.bytes = (size_t)s.blk * s.parts * a.batch * a.n_kv_head * 2 * kT * a.head_dim * sizeof(float);
+  return s;
+}
+size_t sink_parts_offset(const TyrAttnBackwardArgs& a) {
+  return (backward_workspace_bytes(a.batch, a.n_head, a.q_seq) + 255) & ~(size_t)255;
+}
+
+template <int D, bool kSink>
+int launch_bwd(const TyrAttnBackwardArgs& a, int n_sink, float scale, int* status, cudaStream_t st) {
   using C = BCfg<D>;
   const int n_qblk = (a.q_seq + kT - 1) / kT, n_kblk = (a.kv_seq + kT - 1) / kT;
   const int sq_pad = n_qblk * kT;
@@ -1079,12 +1188,12 @@ int launch_bwd(const TyrAttnBackwardArgs& a, float scale, int* status, cudaStrea
     static std::atomic<bool> attr_set[64] = {};
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -TYR_ATTN_ERR_NO_DEVICE;
     if (!attr_set[dev].load(std::memory_order_acquire)) {
-      cudaError_t e = cudaFuncSetAttribute(bwd_dkdv_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      cudaError_t e = cudaFuncSetAttribute(bwd_dkdv_kernel<D, false, kSink>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            (int)C::kSmemBytes);
       if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(bwd_dkdv_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmemBytes);
+        e = cudaFuncSetAttribute(bwd_dkdv_kernel<D, true, kSink>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmemBytes);
       if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(bwd_dq_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        e = cudaFuncSetAttribute(bwd_dq_kernel<D, kSink>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)DqCfg<D>::kSmemBytes);
       if (e != cudaSuccess) return (int)e;
       attr_set[dev].store(true, std::memory_order_release);
@@ -1126,14 +1235,9 @@ int launch_bwd(const TyrAttnBackwardArgs& a, float scale, int* status, cudaStrea
   p.status = status;
   p.wait_limit = wait_limit_cycles();
 
-  int sms = 148;
-  {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
-      sms = 148;
-  }
-  const long long grid_kv = (long long)n_kblk * a.n_kv_head * a.batch;
+  const int sms = sms_of_device();
+  const SinkPlan sink = kSink ? sink_plan(a, n_sink, sms) : SinkPlan{0, 1, 0};
+  const long long grid_kv = (long long)(n_kblk + sink.blk * (sink.parts - 1)) * a.n_kv_head * a.batch;
   const long long grid_q = (long long)n_qblk * a.n_head * a.batch;
   if (grid_kv > 0x7fffffffLL || grid_q > 0x7fffffffLL) return -TYR_ATTN_ERR_TOO_LARGE;
 
@@ -1144,16 +1248,26 @@ int launch_bwd(const TyrAttnBackwardArgs& a, float scale, int* status, cudaStrea
     p.out2_stride[i] = a.dv_stride[i];
   }
   p.wait_first = 0;
-  p.parts = unit_parts<D>(p, dev, sms);
+  p.n_sink = n_sink;
+  p.sink_blk = sink.blk;
+  p.sink_parts = 1;
+  p.sink_out = nullptr;
+  p.parts = unit_parts<D, kSink>(p, dev, sms);
+  if (kSink && p.parts == 1 && sink.parts > 1) {  // (the CTAs of a cluster share a long unit by themselves)
+    p.sink_parts = sink.parts;
+    p.sink_out = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + sink_parts_offset(a));
+  }
+  const long long units_kv = p.sink_parts > 1 ? grid_kv : (long long)n_kblk * a.n_kv_head * a.batch;
   cudaError_t e = p.parts > 1
-                      ? launch_overlapped(bwd_dkdv_kernel<D, true>, dim3((unsigned)(grid_kv * p.parts)), dim3(kBwdThreads),
+                      ? launch_overlapped(bwd_dkdv_kernel<D, true, kSink>, dim3((unsigned)(units_kv * p.parts)), dim3(kBwdThreads),
                                           C::kSmemBytes, st, (unsigned)p.parts, tk, tv, tq, tdo, p)
-                      : launch_overlapped(bwd_dkdv_kernel<D, false>, dim3((unsigned)std::min<long long>(grid_kv, sms)),
+                      : launch_overlapped(bwd_dkdv_kernel<D, false, kSink>, dim3((unsigned)std::min<long long>(units_kv, sms)),
                                           dim3(kBwdThreads), C::kSmemBytes, st, 1, tk, tv, tq, tdo, p);
   count_launch();
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
 
+  const BwdParams of_keys = p;
   p.out1 = static_cast<__nv_bfloat16*>(a.d_q);
   p.out2 = nullptr;
   for (int i = 0; i < 3; ++i) {
@@ -1170,8 +1284,15 @@ int launch_bwd(const TyrAttnBackwardArgs& a, float scale, int* status, cudaStrea
                            span(a.k, a.n_kv_head, a.kv_seq, a.k_stride), span(a.v, a.n_kv_head, a.kv_seq, a.v_stride)})
       if (out.first < in.second && in.first < out.second) p.wait_first = 1;
   }
-  e = launch_overlapped(bwd_dq_kernel<D>, dim3((unsigned)std::min<long long>(grid_q, sms)), dim3(kBwdThreads),
+  e = launch_overlapped(bwd_dq_kernel<D, kSink>, dim3((unsigned)std::min<long long>(grid_q, sms)), dim3(kBwdThreads),
                         DqCfg<D>::kSmemBytes, st, 1, tq, tdo, tk, tv, p);
+  count_launch();
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (!kSink || of_keys.sink_parts == 1 || e != cudaSuccess) return (int)e;
+  // (the dQ kernel is complete only when the dK/dV kernel is)
+  const int64_t quads = (int64_t)sink.blk * a.batch * a.n_kv_head * 2 * kT * (D / 4);
+  if ((quads + 255) / 256 > 0x7fffffffLL) return -TYR_ATTN_ERR_TOO_LARGE;
+  e = launch_overlapped(bwd_sink_merge_kernel<D>, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, 1, of_keys);
   count_launch();
   return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
@@ -1183,10 +1304,15 @@ size_t backward_workspace_bytes(int batch, int n_head, int q_seq) {
   return (size_t)(2 * (int64_t)batch * n_head * sq_pad * (int64_t)sizeof(float));
 }
 
-int launch_backward_sm100(const TyrAttnBackwardArgs& a, float scale, int* status, cudaStream_t st) {
-  if (a.head_dim == 128) return launch_bwd<128>(a, scale, status, st);
-  if (a.head_dim == 64) return launch_bwd<64>(a, scale, status, st);
-  return -TYR_ATTN_ERR_HEAD_DIM;
+size_t backward_sinks_workspace_bytes(const TyrAttnBackwardArgs& a, int n_sink) {
+  const SinkPlan s = sink_plan(a, n_sink, sms_of_device());
+  return s.bytes ? sink_parts_offset(a) + s.bytes : backward_workspace_bytes(a.batch, a.n_head, a.q_seq);
+}
+
+int launch_backward_sm100(const TyrAttnBackwardArgs& a, int n_sink, float scale, int* status, cudaStream_t st) {
+  if (a.head_dim != 64 && a.head_dim != 128) return -TYR_ATTN_ERR_HEAD_DIM;
+  if (n_sink > 0) return a.head_dim == 128 ? launch_bwd<128, true>(a, n_sink, scale, status, st) : launch_bwd<64, true>(a, n_sink, scale, status, st);
+  return a.head_dim == 128 ? launch_bwd<128, false>(a, 0, scale, status, st) : launch_bwd<64, false>(a, 0, scale, status, st);
 }
 
 }  // namespace tyr

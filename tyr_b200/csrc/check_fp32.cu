@@ -29,6 +29,7 @@ struct CheckParams {
   const uint8_t* key_mask;  // [batch, kv_seq], 0 = padding key; or null
   int64_t key_mask_stride;
   float scale;
+  int n_sink;  // keys before it stay visible beside the window
 };
 
 template <typename T>
@@ -58,10 +59,12 @@ check_kernel(const CheckParams p) {
 #pragma unroll
   for (int x = 0; x < kMaxD / 32; ++x) acc[x] = 0.f;
 
-  for (int k0 = key_lo; k0 < n_keys; k0 += 32) {
+  const int n_first = min(p.n_sink, key_lo);  // first tokens in front of the window
+  for (int k0 = n_first > 0 ? 0 : key_lo; k0 < n_keys; k0 = k0 < n_first && k0 + 32 >= n_first ? key_lo : k0 + 32) {
     const int key = k0 + lane;
+    const int end = k0 < n_first ? n_first : n_keys;
     float s = -INFINITY;
-    const bool seen = key < n_keys && (p.key_mask == nullptr || p.key_mask[b * p.key_mask_stride + key] != 0);
+    const bool seen = key < end && (p.key_mask == nullptr || p.key_mask[b * p.key_mask_stride + key] != 0);
     if (seen) {
       const T* kr = kbase + (int64_t)key * p.ks[2];
       float dot = 0.f;
@@ -83,7 +86,7 @@ check_kernel(const CheckParams p) {
     float part[kMaxD / 32];
 #pragma unroll
     for (int x = 0; x < kMaxD / 32; ++x) part[x] = 0.f;
-    const int nk = min(32, n_keys - k0);
+    const int nk = min(32, end - k0);
     for (int kk = 0; kk < nk; ++kk) {
       const float pk = __shfl_sync(0xffffffffu, pr, kk);
       const T* vr = vbase + (int64_t)(k0 + kk) * p.vs[2];
@@ -110,7 +113,7 @@ check_kernel(const CheckParams p) {
 
 }  // namespace
 
-int launch_prefill_check(const TyrAttnPrefillArgs& a, float scale, cudaStream_t st) {
+int launch_prefill_check(const TyrAttnPrefillArgs& a, int n_sink, float scale, cudaStream_t st) {
   if (a.head_dim > kMaxD) return -TYR_ATTN_ERR_HEAD_DIM;
   CheckParams p;
   p.q = a.q; p.k = a.k; p.v = a.v; p.o = a.o; p.lse = a.lse;
@@ -124,6 +127,7 @@ int launch_prefill_check(const TyrAttnPrefillArgs& a, float scale, cudaStream_t 
     p.qs[i] = a.q_stride[i]; p.ks[i] = a.k_stride[i]; p.vs[i] = a.v_stride[i]; p.os[i] = a.o_stride[i];
   }
   p.scale = scale;
+  p.n_sink = n_sink;
   const int64_t rows = (int64_t)a.batch * a.n_head * a.q_seq;
   const int64_t blocks = (rows + kWarpsPerBlock - 1) / kWarpsPerBlock;
   if (blocks > 0x7fffffffLL) return -TYR_ATTN_ERR_TOO_LARGE;

@@ -100,6 +100,8 @@ struct PrefillParams {
   // (key-split, continued: kept behind the fields above so that their offsets stay what they were)
   int n_parts;
   FastDiv by_parts;
+  // First tokens that stay visible beside a window (kSinkMask only): how many, and the KV tiles they lie in
+  int n_sink, sink_tiles;
 };
 
 template <int D>
@@ -162,13 +164,19 @@ struct Item {
   int mblk, b, hkv;
   int hq[2];   // query head of Q tile 0 / 1
   int row[2];  // first query row of Q tile 0 / 1
-  int lo;      // first KV tile of the item (> 0 under a sliding window and for the second half of a split item)
+  int lo;      // first KV tile of the item (> 0 under a sliding window and for the second half of a split item);
+               // kSinkMask: KV tiles that no row of the item sees, behind the p.sink_tiles first ones
   int n0, n1;  // KV tiles Q tile 0 / Q tile 1 visit, counted from `lo`
   int part_slot;  // -1, or (part of the keys this work item covers) * n_split + index among the split items
 };
-// Masks compiled into a kernel beyond the causal one: none, the sliding window, or the padding mask (with
-// or without a window).
-constexpr int kNoMask = 0, kWindowMask = 1, kKeyMask = 2;
+// Masks compiled into a kernel beyond the causal one: none, the sliding window, the padding mask (with
+// or without a window), or the sliding window beside first tokens that stay visible.
+constexpr int kNoMask = 0, kWindowMask = 1, kKeyMask = 2, kSinkMask = 3;
+// The j-th KV tile an item visits: the tiles of the first tokens, then those of the window.  Where the two meet, lo is 0.
+template <int kMask>
+__device__ __forceinline__ int tile_at(int lo, int j, int sink_tiles) {
+  return kMask == kSinkMask && j < sink_tiles ? j : lo + j;
+}
 // Two ways to fill the two Q-tile slots of an item:
 //  rows  : 256 consecutive rows of one query head (tile 1 sits 128 rows below tile 0);
 //  heads : the same 128 rows of two query heads that share a KV head (GQA).  Both tiles
@@ -218,6 +226,7 @@ __device__ __forceinline__ Item decode_item(int w, const PrefillParams& p) {
     it.hq[0] = it.hq[1] = it.hkv * p.group + hl;
     it.row[0] = it.row[1] = it.mblk * kBM;
     it.lo = (kMask != kNoMask && p.window > 0) ? max(0, it.row[0] - p.window + 1) / kBN : 0;
+    if (kMask == kSinkMask) it.lo = max(0, it.lo - p.sink_tiles);
     const int n = (p.causal ? min(nkv_total, it.mblk + 1) : nkv_total) - it.lo;
     it.n0 = (n + 1) >> 1;  // tiles 0, 2, ..
     it.n1 = n >> 1;        // tiles 1, 3, ..
@@ -240,6 +249,7 @@ __device__ __forceinline__ Item decode_item(int w, const PrefillParams& p) {
   // Q tiles start at that tile; a tile that lies wholly before a row's window is masked
   // out for that row (the softmax copes with rows that have seen no key yet).
   it.lo = (kMask != kNoMask && p.window > 0) ? max(0, it.row[0] - p.window + 1) / kBN : 0;
+  if (kMask == kSinkMask) it.lo = max(0, it.lo - p.sink_tiles);
   it.n0 = (p.causal ? min(nkv_total, last0) : nkv_total) - it.lo;
   it.n1 = (p.causal ? min(nkv_total, last1) : nkv_total) - it.lo;
   return it;
@@ -512,7 +522,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 #pragma unroll
             for (int kb = 0; kb < C::kBoxes; ++kb)
               tma_load_4d(sK + s * C::kTileBytes + kb * C::kBoxBytes, &tm_k, bar(B::k_full + s), kb * 64,
-                          (im.lo + j) * kBN, im.hkv, im.b);
+                          tile_at<kMask>(im.lo, j, p.sink_tiles) * kBN, im.hkv, im.b);
             ++kc;
           };
           auto load_v = [&](int j) {
@@ -523,7 +533,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 #pragma unroll
             for (int kb = 0; kb < C::kBoxes; ++kb)
               tma_load_4d(sV + s * C::kTileBytes + kb * C::kBoxBytes, &tm_v, bar(B::v_full + s), kb * 64,
-                          (im.lo + j) * kBN, im.hkv, im.b);
+                          tile_at<kMask>(im.lo, j, p.sink_tiles) * kBN, im.hkv, im.b);
             ++vc;
           };
           if (ok) ok = cut_to_keys(im, it, false);
@@ -762,7 +772,9 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       float m_ref = -INFINITY, l = 0.f;
 
       for (int j = j_begin; j < j_end; j += j_step, ++sc) {
-        const int key0 = kRefByRow ? j : (im.lo + j) * kBN;  // first key of the tile
+        // first key of the tile
+        const int key0 = !kRefByRow ? (im.lo + j) * kBN
+                         : kMask == kSinkMask && j < (im.lo + p.sink_tiles) * kBN ? j - im.lo * kBN : j;
         // padding keys: lane i fetches the mask bytes of keys i, 32 + i, 64 + i, 96 + i of the tile, before
         // the wait for the scores, where the warp has time
         uint32_t valid4 = 0;
@@ -788,7 +800,15 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         int limit = p.kv_seq - key0;
         if (p.causal) limit = min(limit, row + 1 - key0);
         const int first = (kMask != kNoMask && p.window > 0) ? row - p.window + 1 - key0 : 0;
-        if (limit < kBN || first > 0) {
+        if (kMask == kSinkMask) {
+          // ... and [0, shown), the first tokens
+          const int shown = p.n_sink - key0;
+          if (limit < kBN || first > 0) {
+#pragma unroll
+            for (int c = 0; c < kBN; ++c)
+              if (c >= limit || (c < first && c >= shown)) sr[c >> 5][c & 31] = 0xff800000u;  // -inf
+          }
+        } else if (limit < kBN || first > 0) {
 #pragma unroll
           for (int c = 0; c < kBN; ++c)
             if (c >= limit || c < first) sr[c >> 5][c & 31] = 0xff800000u;  // -inf
@@ -1120,7 +1140,7 @@ SplitPlan split_plan(const TyrAttnPrefillArgs& a, int n_sm) {
 // two.  One prompt of 517 rows, 32 heads of 128: 80 items of up to 5 steps become 160 of up to 3, 16.4 ->
 // 14.4 us; 1024 rows, 16 heads 22.5 -> 16.4 us; 40 rows on 700 keys 17.2 -> 12.3 us; with a window of 64,
 // 2 x 500 rows, 12 heads of 64 12.1 -> 8.0 us, of 1000, 1000 rows, 6 heads of 64 18.0 -> 11.7 us.
-bool halves_pay(const TyrAttnPrefillArgs& a, int n_sm) {
+bool halves_pay(const TyrAttnPrefillArgs& a, int sink_tiles, int n_sm) {
   if (a.key_mask != nullptr) return false;
   const int nkv = (a.kv_seq + kBN - 1) / kBN, n_mblk = (a.q_seq + kBM - 1) / kBM;
   const long long per_level = (long long)a.n_head * a.batch, items = per_level * n_mblk;
@@ -1128,7 +1148,7 @@ bool halves_pay(const TyrAttnPrefillArgs& a, int n_sm) {
   if (items > 2ll * n_sm || split_plan(a, n_sm).items > n_sm) return false;
   auto tiles = [&](long long w) {  // KV tiles of item w, longest first
     const int mblk = n_mblk - 1 - (int)(w / per_level);
-    const int lo = a.window_size > 0 ? std::max(0, mblk * kBM - a.window_size + 1) / kBN : 0;
+    const int lo = a.window_size > 0 ? std::max(0, std::max(0, mblk * kBM - a.window_size + 1) / kBN - sink_tiles) : 0;
     return (a.is_causal || a.window_size > 0 ? std::min<int>(nkv, mblk + 1) : nkv) - lo;
   };
   auto cost = [&](long long w) { return 2 * ((tiles(w) + 1) / 2) + 2; };
@@ -1270,13 +1290,13 @@ bool overlaps_predecessor(const PrefillParams& p, int head_dim, long long items,
   const int nkv = (p.kv_seq + kBN - 1) / kBN, rows = p.pair_heads ? kBM : 2 * kBM;
   long long tiles = nkv;  // of an average item
   if (p.causal) tiles = std::min<long long>(tiles, ((long long)p.n_mblk * rows / kBN + 1) / 2);
-  if (p.window > 0) tiles = std::min<long long>(tiles, (p.window + rows + kBN - 1) / kBN);
+  if (p.window > 0) tiles = std::min<long long>(tiles, (p.window + rows + kBN - 1) / kBN + p.sink_tiles);
   const int steps = head_dim == 64 || !p.causal ? 40 : !p.pair_heads ? 28 : p.key_mask != nullptr ? 20 : 18;
   return items * tiles <= (long long)steps * n_sm;
 }
 
 template <int D, int kMask>
-int launch(const TyrAttnPrefillArgs& a, float scale, int* status, cudaStream_t st) {
+int launch(const TyrAttnPrefillArgs& a, int n_sink, float scale, int* status, cudaStream_t st) {
   using C = Cfg<D>;
   CUtensorMap tq, tk, tv, to;
   int rc;
@@ -1325,8 +1345,9 @@ int launch(const TyrAttnPrefillArgs& a, float scale, int* status, cudaStream_t s
     sp = split_plan(a, sm_count());
     if (a.workspace_bytes < sp.bytes || (reinterpret_cast<uintptr_t>(a.workspace) & 255) != 0) sp.n_split = 0;
   }
+  const long long sink_tiles = kMask == kSinkMask ? ((long long)std::min(n_sink, a.kv_seq) + kBN - 1) / kBN : 0;
   const bool halves = kMask != kKeyMask && sp.n_split == 0 &&
-                      4ll * a.kv_seq * D * a.batch * a.n_kv_head <= kOneChunkBytes && halves_pay(a, sm_count());
+                      4ll * a.kv_seq * D * a.batch * a.n_kv_head <= kOneChunkBytes && halves_pay(a, (int)sink_tiles, sm_count());
   {
     const int group = a.n_head / a.n_kv_head;
     // pair two heads of a KV head when that removes idle slots: causal masks, short query blocks
@@ -1362,6 +1383,8 @@ int launch(const TyrAttnPrefillArgs& a, float scale, int* status, cudaStream_t s
   p.group = a.n_head / a.n_kv_head;
   p.causal = (a.is_causal || a.window_size > 0) ? 1 : 0;
   p.window = a.window_size > 0 ? a.window_size : 0;
+  p.n_sink = n_sink;
+  p.sink_tiles = (int)sink_tiles;
   p.key_mask = a.key_mask;
   p.key_mask_stride = a.key_mask_stride;
   p.scale_log2 = scale * 1.4426950408889634f;
@@ -1438,12 +1461,13 @@ long long prefill_split_workspace_bytes(const TyrAttnPrefillArgs& a) {
   return split_plan(a, sm_count()).bytes;
 }
 
-int launch_prefill_sm100(const TyrAttnPrefillArgs& a, float scale, int* status, cudaStream_t st) {
+int launch_prefill_sm100(const TyrAttnPrefillArgs& a, int n_sink, float scale, int* status, cudaStream_t st) {
   if (a.head_dim != 64 && a.head_dim != 128) return -TYR_ATTN_ERR_HEAD_DIM;
   const bool wide = a.head_dim == 128;
-  if (a.key_mask != nullptr) return wide ? launch<128, kKeyMask>(a, scale, status, st) : launch<64, kKeyMask>(a, scale, status, st);
-  if (a.window_size > 0) return wide ? launch<128, kWindowMask>(a, scale, status, st) : launch<64, kWindowMask>(a, scale, status, st);
-  return wide ? launch<128, kNoMask>(a, scale, status, st) : launch<64, kNoMask>(a, scale, status, st);
+  if (a.key_mask != nullptr) return wide ? launch<128, kKeyMask>(a, 0, scale, status, st) : launch<64, kKeyMask>(a, 0, scale, status, st);
+  if (n_sink > 0) return wide ? launch<128, kSinkMask>(a, n_sink, scale, status, st) : launch<64, kSinkMask>(a, n_sink, scale, status, st);
+  if (a.window_size > 0) return wide ? launch<128, kWindowMask>(a, 0, scale, status, st) : launch<64, kWindowMask>(a, 0, scale, status, st);
+  return wide ? launch<128, kNoMask>(a, 0, scale, status, st) : launch<64, kNoMask>(a, 0, scale, status, st);
 }
 
 }  // namespace tyr

@@ -144,10 +144,16 @@ void fill_prefill(TyrAttnPrefillArgs& a, const Tensor& q, const Tensor& k, const
   a.dtype = dt == at::kBFloat16 ? TYR_ATTN_BF16 : TYR_ATTN_F32;
 }
 
-// q, k, v, is_causal, scale, out, lse, return_lse, check_mode, window_size, key_mask, workspace -> (out, lse)
+// a window or a number of first tokens: beyond any length is as good as the greatest length
+int32_t span_of(PyObject* o) {
+  const int64_t v = integer(o);
+  return v > INT32_MAX ? INT32_MAX : v < 0 ? -1 : static_cast<int32_t>(v);
+}
+
+// q, k, v, is_causal, scale, out, lse, return_lse, check_mode, window_size, key_mask, workspace, n_sink -> (out, lse)
 PyObject* attention_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    require_count(n, 12);
+    require_count(n, 13);
     const Tensor &q = tensor(args[0], "q"), &k = tensor(args[1], "k"), &v = tensor(args[2], "v");
     require_cuda(q);
     require_cuda(k);
@@ -162,7 +168,8 @@ PyObject* attention_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.is_causal = causal;
     a.scale = scale_of(args[4]);
     a.check_mode = check_mode;
-    a.window_size = i32(integer(args[9]));
+    const int32_t n_sink = span_of(args[12]);
+    a.window_size = n_sink != 0 ? span_of(args[9]) : i32(integer(args[9]));
     if (lse_in && (lse_in->scalar_type() != at::kFloat || !lse_in->is_contiguous() || lse_in->dim() != 3 ||
                    lse_in->size(0) != q.size(0) || lse_in->size(1) != q.size(1) || lse_in->size(2) != q.size(2)))
       throw ValueError("lse must be a contiguous float32 [batch, n_head, q_seq] tensor");
@@ -193,7 +200,7 @@ PyObject* attention_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
           a.workspace_bytes = ws.numel();
         }
       }
-      check_rc(tyr_b200_attn_prefill(&a, stream_of(q)));
+      check_rc(n_sink != 0 ? tyr_b200_attn_prefill_sinks(&a, n_sink, stream_of(q)) : tyr_b200_attn_prefill(&a, stream_of(q)));
     }
     PyObject* t = PyTuple_New(2);
     if (!t) throw python_error();
@@ -213,10 +220,10 @@ Tensor like(const Tensor& t) {
   return t.is_contiguous() ? new_tensor(t.sizes(), t.scalar_type(), t.device()) : at::empty_like(t);
 }
 
-// q, k, v, o, lse, d_o, is_causal, scale, workspace, window_size, key_mask -> (d_q, d_k, d_v)
+// q, k, v, o, lse, d_o, is_causal, scale, workspace, window_size, key_mask, n_sink -> (d_q, d_k, d_v)
 PyObject* attention_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    require_count(n, 11);
+    require_count(n, 12);
     const Tensor &q = tensor(args[0], "q"), &k = tensor(args[1], "k"), &v = tensor(args[2], "v"), &o = tensor(args[3], "o"),
                  &lse = tensor(args[4], "lse"), &d_o = tensor(args[5], "d_o");
     for (const Tensor* t : {&q, &k, &v, &o, &d_o, &lse}) require_cuda(*t);
@@ -240,17 +247,20 @@ PyObject* attention_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.dtype = TYR_ATTN_BF16;
     a.is_causal = truth(args[6]);
     a.scale = scale_of(args[7]);
-    a.window_size = i32(integer(args[9]));
+    const int32_t n_sink = span_of(args[11]);
+    a.window_size = n_sink != 0 ? span_of(args[9]) : i32(integer(args[9]));
     if (mask) {
       const Tensor m = key_bytes(*mask, k.size(0), k.size(2));
       a.key_mask = static_cast<const uint8_t*>(m.data_ptr());
       a.key_mask_stride = m.stride(0);
     }
-    const int64_t need = (int64_t)tyr_b200_attn_backward_workspace_bytes(a.batch, a.n_head, a.q_seq);
     Tensor ws, d_q, d_k, d_v;
     {
       NoGil no_gil;
       c10::cuda::OptionalCUDAGuard guard(q.device());
+      const int64_t need = n_sink != 0 ? tyr_b200_attn_backward_sinks_workspace_bytes(&a, n_sink)
+                                       : (int64_t)tyr_b200_attn_backward_workspace_bytes(a.batch, a.n_head, a.q_seq);
+      if (need < 0) throw CallError{(int)need};
       ws = ws_in ? *ws_in : new_tensor({need / 4}, at::kFloat, q.device());
       if (ws.scalar_type() != at::kFloat || !ws.is_contiguous() || ws.numel() * 4 < need)
         throw ValueError("workspace must be a contiguous float32 CUDA tensor of the required size");
@@ -261,7 +271,7 @@ PyObject* attention_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
       strides3(a.dq_stride, d_q); strides3(a.dk_stride, d_k); strides3(a.dv_stride, d_v);
       a.workspace = ws.data_ptr();
       a.workspace_bytes = (uint64_t)ws.numel() * 4;
-      check_rc(tyr_b200_attn_backward(&a, stream_of(q)));
+      check_rc(n_sink != 0 ? tyr_b200_attn_backward_sinks(&a, n_sink, stream_of(q)) : tyr_b200_attn_backward(&a, stream_of(q)));
     }
     PyObject* t = PyTuple_New(3);
     if (!t) throw python_error();
@@ -400,11 +410,6 @@ PyObject* decode_dense(PyObject*, PyObject* const* args, Py_ssize_t n) {
 int32_t count_of(int64_t v, const char* what) {
   if (v < INT32_MIN || v > INT32_MAX) throw ValueError(std::string(what) + " does not fit 32 bits");
   return static_cast<int32_t>(v);
-}
-// a window or a number of first tokens: beyond any length is as good as the greatest length
-int32_t span_of(PyObject* o) {
-  const int64_t v = integer(o);
-  return v > INT32_MAX ? INT32_MAX : v < 0 ? -1 : static_cast<int32_t>(v);
 }
 void same_device(const Tensor& t, const Tensor& as, const char* what) {
   if (!t.is_cuda() || t.device() != as.device()) throw ValueError(std::string(what) + " must be on the device of the other tensors");

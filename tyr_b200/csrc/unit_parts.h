@@ -10,6 +10,7 @@ struct BwdSizes {
   int n_kv, n_q;           // KV heads and query heads of the whole batch
   int group, window;       // query heads per KV head; 0: no window
   bool causal;
+  int sink_blk = 0;        // key blocks that every query row sees beside the window
 };
 constexpr int kMaxPlanSms = 256;
 constexpr int kPartsChoices = 4;  // 1, 2, 4 or 8 CTAs per unit
@@ -31,12 +32,12 @@ inline int choose_unit_parts(const BwdSizes& z, int sms, const int* capacity) {
   constexpr int kPair = 5, kDqPair = 4;
   auto pairs_of_keys = [&](int blk) {    // streamed pairs of a unit
     const int lo = z.causal ? std::min(blk, z.n_qblk) : 0;
-    const int hi = z.window > 0 ? std::min(z.n_qblk, (blk * 128 + 127 + z.window - 1) / 128 + 1) : z.n_qblk;
+    const int hi = z.window > 0 && blk >= z.sink_blk ? std::min(z.n_qblk, (blk * 128 + 127 + z.window - 1) / 128 + 1) : z.n_qblk;
     return std::max(hi - lo, 0) * z.group;
   };
   auto pairs_of_rows = [&](int blk) {    // KV tiles of a dQ unit
     const int hi = z.causal ? std::min(z.n_kblk, blk + 1) : z.n_kblk;
-    const int lo = z.window > 0 ? std::max(0, blk * 128 - z.window + 1) / 128 : 0;
+    const int lo = z.window > 0 ? std::max(0, std::max(0, blk * 128 - z.window + 1) / 128 - z.sink_blk) : 0;
     return std::max(hi - lo, 0);
   };
   const long long units = (long long)z.n_kblk * z.n_kv, row_units = (long long)z.n_qblk * z.n_q;
@@ -85,6 +86,19 @@ inline int choose_unit_parts(const BwdSizes& z, int sms, const int* capacity) {
     }
   }
   return best_parts;
+}
+
+// First keys that every query row sees beside a window: a unit of theirs streams all query blocks, others a window's.  In how
+// many units, of separate query rows, each of those key blocks is done, so that the longest unit is no
+// longer than another, or than half of what an SM has to do in all.  By the sizes of one batch element, so that the order
+// of its sums does not depend on the batch.
+constexpr int kMaxSinkParts = 64;
+inline int choose_sink_parts(int n_kblk, int n_qblk, int n_kv_head, int group, int window, int sink_blk, int sms) {
+  const long long all = (long long)n_qblk * group;
+  const long long near = std::min<long long>(n_qblk, (127ll + window - 1) / 128 + 1) * group;
+  const long long load = (sink_blk * all + (n_kblk - sink_blk) * near) * n_kv_head / std::max(sms, 1);
+  const long long longest = std::max<long long>(std::max(near, load / 2), 1);
+  return (int)std::min<long long>(std::max<long long>((all + longest - 1) / longest, 1), std::min<long long>(kMaxSinkParts, (long long)std::max(n_qblk - sink_blk + 1, 1) * group));
 }
 
 }  // namespace tyr

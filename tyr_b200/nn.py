@@ -71,7 +71,7 @@ def attentionFwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, is_causal: b
                  lse: Optional[torch.Tensor] = None, return_lse: bool = True,
                  check_mode: bool = False, window_size: int = 0,
                  key_mask: Optional[torch.Tensor] = None,
-                 workspace=None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+                 workspace=None, n_sink: int = 0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """O = softmax(Q K^T * scale + causal) V and the per-row LSE.
 
     q [B,Hq,Sq,D]; k, v [B,Hkv,Skv,D] (Hq % Hkv == 0, query head h reads KV head
@@ -80,6 +80,8 @@ def attentionFwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, is_causal: b
     Tyr/Model/Qwen/Attention.lean:195-196.  `check_mode` runs the fp32-FMA kernel.
     `window_size` > 0 adds the causal sliding window of lean_torch_sdpa_gqa_window
     (cc/src/tyr.cpp:3986-3996): key j is visible to query i only if j <= i and i - j < window_size.
+    `n_sink` > 0 (with a window, without `key_mask`) keeps the first `n_sink` keys visible beside it: key j is visible to
+    query i when j <= i and (i - j < window_size or j < n_sink).
     `key_mask` (uint8 / bool CUDA tensor [batch, kv_seq], 0 = padding key) hides padding keys
     from every query, the key side of lean_torch_sdpa_gqa_mask (cc/src/tyr.cpp:4063-4086).
     Launcher convention of Examples/GPU/RunFlashAttn.lean:68-81: outputs may be
@@ -89,7 +91,7 @@ def attentionFwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, is_causal: b
     one, it is allocated if none is given (`workspace=False`: one launch without any).
     """
     return _lib.calls().attention_fwd(q, k, v, is_causal, scale, out, lse, return_lse, check_mode, window_size,
-                                      key_mask, workspace)
+                                      key_mask, workspace, n_sink)
 
 
 def prefill_workspace_bytes(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, is_causal: bool = True) -> int:
@@ -102,7 +104,7 @@ def prefill_workspace_bytes(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, i
 def attentionBwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
                  d_o: torch.Tensor, is_causal: bool = True, scale: Optional[float] = None,
                  workspace: Optional[torch.Tensor] = None, window_size: int = 0,
-                 key_mask: Optional[torch.Tensor] = None
+                 key_mask: Optional[torch.Tensor] = None, n_sink: int = 0
                  ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """dQ, dK, dV of `attentionFwd` from dO, the forward's inputs, its output and its LSE.
 
@@ -111,9 +113,22 @@ def attentionBwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Ten
     formulation of Tyr/GPU/Kernels/MhaH100.lean:196-344.  dK and dV of a KV head are summed over
     the query heads that share it.  `workspace` may be a caller-kept float32 CUDA tensor of at
     least `backward_workspace_bytes(...) / 4` elements; one is allocated otherwise.
-    `window_size` and `key_mask` are those of the forward call (sliding window / padding keys).
+    `window_size`, `key_mask` and `n_sink` are those of the forward call (sliding window / padding keys / first tokens);
+    with `n_sink` a given workspace is of `backward_sinks_workspace_bytes(...)` bytes.
     """
-    return _lib.calls().attention_bwd(q, k, v, o, lse, d_o, is_causal, scale, workspace, window_size, key_mask)
+    return _lib.calls().attention_bwd(q, k, v, o, lse, d_o, is_causal, scale, workspace, window_size, key_mask, n_sink)
+
+
+def backward_sinks_workspace_bytes(q: torch.Tensor, k: torch.Tensor, window_size: int, n_sink: int) -> int:
+    """Bytes of `workspace` that `attentionBwd` with first tokens beside a window needs on these tensors."""
+    a = _lib.BackwardArgs()
+    (a.batch, a.n_head, a.q_seq, a.head_dim), (a.n_kv_head, a.kv_seq) = q.shape, k.shape[1:3]
+    a.window_size = max(-1, min(int(window_size), 2 ** 31 - 1))
+    with torch.cuda.device(q.device):
+        n = int(_lib.load().tyr_b200_attn_backward_sinks_workspace_bytes(ctypes.byref(a), max(-1, min(int(n_sink), 2 ** 31 - 1))))
+    if n < 0:
+        raise AttnError(n)
+    return n
 
 
 def _sdpa(q, k, v, dropout_p, is_causal, enable_gqa):
@@ -156,6 +171,20 @@ def scaledDotProductAttentionGQAWindow(query, key, value, dropout_p: float = 0.0
     if query.shape[2] != key.shape[2]:
         raise ValueError("scaledDotProductAttentionGQAWindow needs q_seq == kv_seq")
     out, _ = attentionFwd(query, key, value, is_causal=True, return_lse=False, window_size=window_size)
+    return out
+
+
+def scaledDotProductAttentionGQAWindowSinks(query, key, value, dropout_p: float = 0.0, is_causal: bool = True,
+                                            enable_gqa: bool = False, window_size: int = 1, n_sink: int = 0):
+    """`scaledDotProductAttentionGQAWindow` with the first `n_sink` keys visible to every query behind them; no
+    counterpart in the reference.  As there, the mask is always causal whatever `is_causal` says."""
+    if dropout_p != 0.0:
+        raise AttnError(-6)
+    if (not enable_gqa and query.shape[1] != key.shape[1]) or window_size <= 0 or n_sink < 0:
+        raise AttnError(-2)
+    if query.shape[2] != key.shape[2]:
+        raise ValueError("scaledDotProductAttentionGQAWindowSinks needs q_seq == kv_seq")
+    out, _ = attentionFwd(query, key, value, is_causal=True, return_lse=False, window_size=window_size, n_sink=n_sink)
     return out
 
 
