@@ -467,6 +467,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         // and 1, which belong to different warps of the pair: the two meet once both hold their
         // columns in registers.  P stays in registers as fp32 for dS.
         uint32_t pr2[2][32];
+        uint32_t dead = 0;  // kSink: bit `step`: P and dS of this warp's chunk are zero
 #pragma unroll
         for (int step = 0; step < 2; ++step) tmem_ld32(tS + (2 * step + half) * 32, pr2[step]);
         tmem_wait_ld();
@@ -479,12 +480,26 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         for (int step = 0; step < 2; ++step) {
           const int c = 2 * step + half;
           uint32_t(&sr)[32] = pr2[step];
-          if (masked) {
+          if (kSink && masked) {
+            // as bits; a chunk that no key row of the warp is seen by needs no exponentials
+            const uint32_t bits = ~bits_below(c_first - 32 * c) & bits_below(c_limit - 32 * c);
+            if (__all_sync(0xffffffffu, bits == 0u)) {
+              dead |= 1u << step;
+            } else {
+#pragma unroll
+              for (int x = 0; x < 32; ++x)
+                if (!(bits & (1u << x))) sr[x] = 0xff800000u;  // -inf: P = 0
+            }
+          } else if (masked) {
 #pragma unroll
             for (int x = 0; x < 32; ++x)
               if (c * 32 + x < c_first || c * 32 + x >= c_limit) sr[x] = 0xff800000u;  // -inf: P = 0
           }
           uint32_t pk_p[16];
+          if (kSink && ((dead >> step) & 1u)) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) pk_p[x] = 0u;
+          } else
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
             // statistics of the two query columns (every lane reads the same addresses)
@@ -539,6 +554,10 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
           uint32_t(&pr)[32] = pr2[step];
           uint32_t(&dp)[32] = dp2[step];
           uint32_t pk_s[16];
+          if (kSink && ((dead >> step) & 1u)) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) pk_s[x] = 0u;
+          } else
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
             const float2 d = *reinterpret_cast<const float2*>(nd_col + c * 32 + 2 * x);
@@ -938,7 +957,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         // padding keys: lane l fetches the mask bytes of keys 2l, 2l+1 of this warp's 64 columns, two
         // ballots spread them to every row; column j of the 64 is bit (j >> 1) of ballot (j & 1)
         uint32_t vb[2] = {0xffffffffu, 0xffffffffu};
-        if (p.key_mask != nullptr) {
+        if (!kSink && p.key_mask != nullptr) {
           const uint8_t* mrow = p.key_mask + w.b * p.key_mask_stride + col0 + 64 * half;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -953,13 +972,26 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           const int c = 2 * half + step;
           uint32_t(&sr)[32] = sr2[step];
           uint32_t(&dp)[32] = dp2[step];
-          if (masked) {
+          bool dead = false;  // kSink: no row of the warp sees a key of the chunk
+          if (kSink && masked) {
+            const uint32_t bits = bits_below(c_limit - 32 * c) & (~bits_below(c_first - 32 * c) | bits_below(c_shown - 32 * c));
+            dead = __all_sync(0xffffffffu, bits == 0u);
+            if (!dead) {
+#pragma unroll
+              for (int x = 0; x < 32; ++x)
+                if (!(bits & (1u << x))) sr[x] = 0xff800000u;  // -inf: P = 0
+            }
+          } else if (masked) {
 #pragma unroll
             for (int x = 0; x < 32; ++x)
-              if (c * 32 + x >= c_limit || (c * 32 + x < c_first && (!kSink || c * 32 + x >= c_shown)) || !((vb[x & 1] >> ((32 * step + x) >> 1)) & 1u))
+              if (c * 32 + x >= c_limit || c * 32 + x < c_first || !((vb[x & 1] >> ((32 * step + x) >> 1)) & 1u))
                 sr[x] = 0xff800000u;  // -inf: P = 0
           }
           uint32_t pk_s[16];
+          if (dead) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) pk_s[x] = 0u;
+          } else
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
             const uint64_t t2 = fma_f32x2(pack_u32x2(sr[2 * x], sr[2 * x + 1]), sl2x2, nl2);

@@ -78,6 +78,7 @@ struct PagedParams : DecodeParams {
   int64_t table_stride;
   FastDiv by_page;
   int n_pages, max_len, window, n_sink;
+  int one_layout;     // K and V have the same strides
   float* ws_scores;   // [batch, n_head, max_kv_seq] scores in the log2 domain, for the running sums of the weights; or null
 };
 template <class P>
@@ -217,8 +218,9 @@ decode_kernel(const __grid_constant__ P p) {
   const int quad = lane >> 2, t4 = lane & 3;
 
   // ---- paged cache: where the rows of a tile lie.  The kLoads rows a thread loads a piece of are the same for the
-  // kChunksPerRow lanes of its group, so each lane looks one of them up, a tile ahead of the loads, and the lanes
-  // exchange what they found: a table entry's latency is not on the path of the loads.
+  // kChunksPerRow lanes of its group, so each lane looks one of them up, a tile ahead of the loads, and the lanes exchange
+  // the offsets: neither a table entry's latency (nothing looks at it before the loads need it) nor a 64-bit
+  // product for every piece is on the path of the loads.
   constexpr int kLoads = kTileKeys * C::kChunksPerRow / kThreads, kRowStep = kThreads / C::kChunksPerRow;
   struct Where { int page, row; };
   bool bad_page = false;
@@ -231,10 +233,6 @@ decode_kernel(const __grid_constant__ P p) {
       const int at = p.by_page.div(key);
       w.row = key - at * (int)p.by_page.d;
       w.page = p.table[b * p.table_stride + at];
-      if ((unsigned)w.page >= (unsigned)p.n_pages) {  // not followed
-        bad_page = true;
-        w.page = 0;
-      }
     }
     return w;
   };
@@ -243,15 +241,24 @@ decode_kernel(const __grid_constant__ P p) {
   auto load_tile = [&](int tile, int stage, Where where) {
     const uint32_t sk = sbase + stage * C::kStageBytes, sv = sk + C::kTileBytes;
     const int k0 = key_begin + tile * kTileKeys;
+    long long at_k = 0, at_v = 0;
+    if constexpr (kPaged) {
+      if ((unsigned)where.page >= (unsigned)p.n_pages) {  // not followed
+        bad_page = true;
+        where.page = 0;
+      }
+      at_k = where.page * p.ks[0] + where.row * p.ks[2];
+      at_v = p.one_layout ? at_k : where.page * p.vs[0] + where.row * p.vs[2];
+    }
 #pragma unroll
     for (int it = 0; it < kLoads; ++it) {
       const int idx = it * kThreads + tid;
       const int kr = idx / C::kChunksPerRow, c = idx % C::kChunksPerRow;
       if constexpr (kPaged) {
-        const int64_t page = __shfl_sync(0xffffffffu, where.page, it, C::kChunksPerRow);
-        const int64_t row = __shfl_sync(0xffffffffu, where.row, it, C::kChunksPerRow);
-        cp_async16(sk + sw_off<D>(kr, c), kbase + page * p.ks[0] + row * p.ks[2] + c * 8);
-        cp_async16(sv + sw_off<D>(kr, c), vbase + page * p.vs[0] + row * p.vs[2] + c * 8);
+        const long long k_at = __shfl_sync(0xffffffffu, at_k, it, C::kChunksPerRow);
+        const long long v_at = p.one_layout ? k_at : __shfl_sync(0xffffffffu, at_v, it, C::kChunksPerRow);
+        cp_async16(sk + sw_off<D>(kr, c), kbase + c * 8 + k_at);
+        cp_async16(sv + sw_off<D>(kr, c), vbase + c * 8 + v_at);
         continue;
       }
       const int key = min(k0 + kr, key_end - 1);  // rows past the end re-read the last valid key
@@ -821,6 +828,7 @@ int launch_paged_decode(const TyrAttnPagedDecodeArgs& a, float scale, int* statu
   p.max_len = a.max_kv_seq;
   p.window = a.window_size;
   p.n_sink = a.n_sink;
+  p.one_layout = a.k_stride[0] == a.v_stride[0] && a.k_stride[2] == a.v_stride[2];
   if ((long long)p.n_kv_head * p.row_groups > 65535) return -TYR_ATTN_ERR_TOO_LARGE;  // (the grid's y extent)
   char* ws = static_cast<char*>(a.workspace);
   p.ws_o = reinterpret_cast<float*>(ws);

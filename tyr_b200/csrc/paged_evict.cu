@@ -46,43 +46,17 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// Exclusive prefix sums of `x` over the CTA's threads, and the total.
-__device__ __forceinline__ uint2 block_scan(uint2 x, uint2* warp_sums, uint2& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint2 s = x;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t a = __shfl_up_sync(0xffffffffu, s.x, o), b = __shfl_up_sync(0xffffffffu, s.y, o);
-    if (lane >= o) {
-      s.x += a;
-      s.y += b;
-    }
-  }
-  if (lane == 31) warp_sums[warp] = s;
-  __syncthreads();
-  uint2 base = make_uint2(0u, 0u);
-  total = make_uint2(0u, 0u);
-#pragma unroll 8
-  for (int w = 0; w < kSelectThreads / 32; ++w) {
-    const uint2 y = warp_sums[w];
-    if (w < warp) {
-      base.x += y.x;
-      base.y += y.y;
-    }
-    total.x += y.x;
-    total.y += y.y;
-  }
-  __syncthreads();  // the sums are the next call's
-  return make_uint2(base.x + s.x - x.x, base.y + s.y - x.y);
-}
+// Positions a CTA holds at once, kItems of them per thread, position x * kSelectThreads + thread as item x.
+constexpr int kItems = 16, kSegment = kItems * kSelectThreads;
 
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
   __shared__ uint32_t hist[256];
-  __shared__ uint2 warp_sums[kSelectThreads / 32];
+  __shared__ uint32_t counts[kItems * kSelectThreads / 32];  // per item and warp, in the order of the positions: over, equal << 16
+  __shared__ uint32_t warp_sums[kSelectThreads / 32];
   __shared__ uint32_t sel_digit, sel_left;
   grid_launch_dependents();
   grid_dependency_wait();
-  const int hkv = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int hkv = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int raw = p.kv_lens[b], n = min(max(raw, 0), p.max_len);
   int32_t* kept = p.kept + ((int64_t)b * p.n_kv_head + hkv) * p.n_keep;
   if (hkv == 0 && tid == 0) {
@@ -96,6 +70,17 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   float* w = p.weights + b * p.w_stride_b + hkv * p.w_stride_h;
   const int lo = p.n_sink, hi = n - p.n_recent;        // the candidates' positions
   const uint32_t m = p.n_keep - p.n_sink - p.n_recent;  // how many of them stay: fewer than there are
+  // a segment's weights stay in registers over all passes where there is only one
+  float x[kItems];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int i = i0 + k * kSelectThreads + tid;
+      x[k] = i < n ? w[i] : 0.f;
+    }
+  };
+  const bool one_segment = n <= kSegment;
+  load(0);
   // T: the m-th greatest; `left`: how many of the keys equal to it stay
   uint32_t T = 0xffffffffu, left = 0;
   if (m > 0) {
@@ -105,18 +90,24 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
       if (tid < 256) hist[tid] = 0;
       __syncthreads();
       const uint32_t above = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-      for (int i = lo + tid; i < hi; i += kSelectThreads) {
-        const uint32_t u = ordered(w[i]);
-        if ((u & above) == T) atomicAdd(&hist[(u >> shift) & 255u], 1u);
+      for (int i0 = 0; i0 < hi; i0 += kSegment) {
+        if (!one_segment) load(i0);
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+          const int i = i0 + k * kSelectThreads + tid;
+          if (i0 + k * kSelectThreads >= hi) break;
+          const uint32_t u = ordered(x[k]);
+          if (i >= lo && i < hi && (u & above) == T) atomicAdd(&hist[(u >> shift) & 255u], 1u);
+        }
       }
       __syncthreads();
       if (tid < 32) {
         // lane l has digits 255 - 8 l .. 248 - 8 l: the greatest first
         uint32_t c[8], sum = 0;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          c[x] = hist[255 - 8 * tid - x];
-          sum += c[x];
+        for (int d = 0; d < 8; ++d) {
+          c[d] = hist[255 - 8 * tid - d];
+          sum += c[d];
         }
         uint32_t before = sum;
 #pragma unroll
@@ -126,12 +117,12 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
         }
         before -= sum;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          if (before < left && before + c[x] >= left) {
-            sel_digit = 255 - 8 * tid - x;
+        for (int d = 0; d < 8; ++d) {
+          if (before < left && before + c[d] >= left) {
+            sel_digit = 255 - 8 * tid - d;
             sel_left = left - before;
           }
-          before += c[x];
+          before += c[d];
         }
       }
       __syncthreads();
@@ -141,31 +132,65 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   }
   // in the order of the positions: a key stays if it always does, weighs more than T, or is one of the first `left` equal to T
   uint32_t over_before = 0, equal_before = 0;
-  for (int i0 = 0; i0 < n; i0 += kSelectThreads) {
-    const int i = i0 + tid;
-    const float x = i < n ? w[i] : 0.f;
-    const uint32_t u = ordered(x);
-    const bool always = i < lo || (i >= hi && i < n), candidate = i >= lo && i < hi;
-    const bool over = always || (candidate && u > T), equal = candidate && u == T;
-    uint2 total;
-    const uint2 before = block_scan(make_uint2(over, equal), warp_sums, total);  // (every weight of the step is in a register behind it)
-    const uint32_t eq = equal_before + before.y;
-    if (over || (equal && eq < left)) {
-      const uint32_t to = over_before + before.x + min(eq, left);
-      kept[to] = i;
-      w[to] = x;
+  for (int i0 = 0; i0 < n; i0 += kSegment) {
+    if (!one_segment) load(i0);
+    uint32_t over_bits = 0, equal_bits = 0;  // of this thread's items
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int i = i0 + k * kSelectThreads + tid;
+      const uint32_t u = ordered(x[k]);
+      const bool candidate = i >= lo && i < hi;
+      const bool over = i < lo || (i >= hi && i < n) || (candidate && u > T), equal = candidate && u == T;
+      over_bits |= (uint32_t)over << k;
+      equal_bits |= (uint32_t)equal << k;
+      const uint32_t c = __popc(__ballot_sync(0xffffffffu, over)) | __popc(__ballot_sync(0xffffffffu, equal)) << 16;
+      if (lane == 0) counts[k * (kSelectThreads / 32) + warp] = c;
     }
-    over_before += total.x;
-    equal_before += total.y;
+    __syncthreads();  // every weight of the segment is in a register, every count in shared memory
+    // exclusive prefix sums of the counts (at most kSegment of either kind: 16 bits each)
+    constexpr int kCounts = kItems * kSelectThreads / 32;
+    static_assert(kCounts <= kSelectThreads && kSegment < 65536, "one count per thread");
+    const uint32_t mine = tid < kCounts ? counts[tid] : 0u;
+    uint32_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    if (lane == 31) warp_sums[warp] = sum;
+    __syncthreads();
+    uint32_t base = 0, total = 0;
+#pragma unroll
+    for (int v = 0; v < kCounts / 32; ++v) {
+      base += v < warp ? warp_sums[v] : 0u;
+      total += warp_sums[v];
+    }
+    if (tid < kCounts) counts[tid] = base + sum - mine;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const bool over = (over_bits >> k) & 1u, equal = (equal_bits >> k) & 1u;
+      const uint32_t lower = (1u << lane) - 1u, c = counts[k * (kSelectThreads / 32) + warp];
+      const uint32_t over_at = over_before + (c & 0xffffu) + __popc(__ballot_sync(0xffffffffu, over) & lower);
+      const uint32_t equal_at = equal_before + (c >> 16) + __popc(__ballot_sync(0xffffffffu, equal) & lower);
+      if (over || (equal && equal_at < left)) {
+        const uint32_t to = over_at + min(equal_at, left);
+        kept[to] = i0 + k * kSelectThreads + tid;
+        w[to] = x[k];  // (at most the key's own position)
+      }
+    }
+    over_before += total & 0xffffu;
+    equal_before += total >> 16;
+    __syncthreads();  // (the counts are the next segment's)
   }
-  __syncthreads();
   for (int i = p.n_keep + tid; i < n; i += kSelectThreads) w[i] = 0.f;
 }
 
-// kLanes threads of 16 bytes make one row of a CTA's columns; kRows rows of each thread are in flight.
+// kLanes threads of 16 bytes make one row of a CTA's columns; kRows rows of each thread are in flight, and the next step's
+// addresses (list entry, then table entry) are on their way while a step's rows arrive.
 template <int kLanes>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p, int slices) {
-  constexpr int kRows = 8, kGroup = kMoveThreads / kLanes;  // rows a step moves: kRows * kGroup
+  constexpr int kRows = 8, kGroup = kMoveThreads / kLanes, kStep = kRows * kGroup;  // kStep: rows a step moves
   grid_launch_dependents();
   grid_dependency_wait();
   const int hkv = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
@@ -173,41 +198,57 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
   if (n <= p.n_keep) return;
   const bool is_v = (int)blockIdx.x >= slices;
   const int col = ((is_v ? blockIdx.x - slices : blockIdx.x) * kLanes + tid % kLanes) * 8;
-  const int64_t* st = is_v ? p.vs : p.ks;
-  __nv_bfloat16* base = (is_v ? p.v : p.k) + hkv * st[1] + col;
+  const int64_t st0 = is_v ? p.vs[0] : p.ks[0], st2 = is_v ? p.vs[2] : p.ks[2];
+  __nv_bfloat16* base = (is_v ? p.v + hkv * p.vs[1] : p.k + hkv * p.ks[1]) + col;
   const int32_t* kept = p.kept + ((int64_t)b * p.n_kv_head + hkv) * p.n_keep;
   const int32_t* table = p.table + b * p.table_stride;
-  auto row_of = [&](int r) -> __nv_bfloat16* {
-    const int at = p.by_page.div(r), id = table[at];
-    if ((unsigned)id >= (unsigned)p.n_pages) return nullptr;  // not followed
-    return base + (int64_t)id * st[0] + (int64_t)(r - at * (int)p.by_page.d) * st[2];
-  };
   bool bad = false;
-  for (int i0 = 0; i0 < p.n_keep; i0 += kRows * kGroup) {
-    uint4 x[kRows];
-    __nv_bfloat16* to[kRows];
+  __nv_bfloat16 *from[kRows], *to[kRows];
+  auto addresses = [&](int i0) {
+    int src[kRows], page_from[kRows], page_to[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const int i = i0 + r * kGroup + tid / kLanes;
-      to[r] = nullptr;
-      if (i >= p.n_keep) continue;
-      const int src = kept[i];
-      if (src == i) continue;  // it lies there
-      const __nv_bfloat16* from = row_of(src);
-      to[r] = row_of(i);
-      if (from == nullptr || to[r] == nullptr) {
-        to[r] = nullptr;
-        bad = true;
-        continue;
-      }
-      x[r] = *reinterpret_cast<const uint4*>(from);
+      src[r] = i < p.n_keep ? kept[i] : i;
     }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const int i = i0 + r * kGroup + tid / kLanes;
+      page_from[r] = src[r] == i ? 0 : table[p.by_page.div(src[r])];  // (a row that stays where it is needs none)
+      page_to[r] = src[r] == i ? 0 : table[p.by_page.div(i)];
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const int i = i0 + r * kGroup + tid / kLanes;
+      const bool out = (unsigned)page_from[r] >= (unsigned)p.n_pages || (unsigned)page_to[r] >= (unsigned)p.n_pages;  // not followed
+      bad = bad || (src[r] != i && out);
+      from[r] = base + page_from[r] * st0 + (src[r] - p.by_page.div(src[r]) * (int)p.by_page.d) * st2;
+      to[r] = src[r] == i || out ? nullptr : base + page_to[r] * st0 + (i - p.by_page.div(i) * (int)p.by_page.d) * st2;
+    }
+  };
+  addresses(0);
+  for (int i0 = 0; i0 < p.n_keep; i0 += kStep) {
+    uint4 x[kRows];
+    __nv_bfloat16* here[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      here[r] = to[r];
+      if (here[r] != nullptr) x[r] = *reinterpret_cast<const uint4*>(from[r]);
+    }
+    if (i0 + kStep < p.n_keep) addresses(i0 + kStep);
     __syncthreads();  // every row of the step is in registers
 #pragma unroll
     for (int r = 0; r < kRows; ++r)
-      if (to[r] != nullptr) *reinterpret_cast<uint4*>(to[r]) = x[r];
+      if (here[r] != nullptr) *reinterpret_cast<uint4*>(here[r]) = x[r];
   }
   if (bad) atomicOr(p.status, kStatusOutOfRange);
+}
+
+// The columns of a row that one CTA moves: 128 bytes, or 32 where those CTAs would not fill the SMs.
+template <int kLanes>
+cudaError_t launch_move(const EvictParams& p, int batch, int head_dim, cudaStream_t st) {
+  const int slices = head_dim / (8 * kLanes);
+  return launch_overlapped(evict_move_kernel<kLanes>, dim3(2 * slices, p.n_kv_head, batch), dim3(kMoveThreads), 0, st, 1, p, slices);
 }
 
 }  // namespace
@@ -238,9 +279,8 @@ int launch_paged_evict(const TyrAttnEvictArgs& a, int* status, cudaStream_t st) 
   count_launch();
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
-  constexpr int kLanes = 8;  // 128 bytes of a row per CTA
-  const int slices = a.head_dim / (8 * kLanes);
-  e = launch_overlapped(evict_move_kernel<kLanes>, dim3(2 * slices, a.n_kv_head, a.batch), dim3(kMoveThreads), 0, st, 1, p, slices);
+  const bool wide = 2ll * (a.head_dim / 64) * a.n_kv_head * a.batch >= 2ll * sm_count();
+  e = wide ? launch_move<8>(p, a.batch, a.head_dim, st) : launch_move<2>(p, a.batch, a.head_dim, st);
   count_launch();
   return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }

@@ -20,6 +20,9 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// bits 0 .. n - 1 of 32 set (none for n <= 0, all for n >= 32)
+__device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? 0xffffffffu : ~(0xffffffffu << max(n, 0)); }
+
 // See launch_overlapped (attn_internal.h).
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
