@@ -66,18 +66,18 @@ def test_refusals(built_lib):
     assert g(None, 1, None) == -1 and need(None, 1) == -1
     assert g(ctypes.byref(a), -1, None) == -2 and need(ctypes.byref(a), -1) == -2
     plain_need = built_lib.tyr_b200_attn_backward_workspace_bytes(1, 4, 8)
-    assert need(ctypes.byref(a), 0) == need(ctypes.byref(a), 2) == plain_need        # one key block: nothing to cut
+    assert need(ctypes.byref(a), 0) == plain_need and plain_need < need(ctypes.byref(a), 2) <= plain_need + 512   # one key block: a counter only
     assert g(ctypes.byref(a), 2, None) == -7
-    a.workspace, a.workspace_bytes = p, plain_need - 1
+    a.workspace, a.workspace_bytes = p, need(ctypes.byref(a), 2) - 1
     assert g(ctypes.byref(a), 2, None) == -7
     a.window_size = 0
     assert g(ctypes.byref(a), 2, None) == -2 and need(ctypes.byref(a), 2) == -2
     a.window_size, a.q_seq, a.kv_seq = 128, 8192, 8192
     base = built_lib.tyr_b200_attn_backward_workspace_bytes(1, 4, 8192)
-    extra = need(ctypes.byref(a), 2) - base
+    extra = need(ctypes.byref(a), 2) - base - 256
     assert extra > 0 and extra % (2 * 2 * 128 * 64 * 4) == 0                         # whole parts of both KV heads
     a.batch = 3
-    assert need(ctypes.byref(a), 2) == 3 * (base + extra)                            # as many parts whatever the batch
+    assert need(ctypes.byref(a), 2) == 3 * (base + extra) + 256                      # as many parts whatever the batch
     a.batch = 0
     assert need(ctypes.byref(a), 2) == 0
     a.batch, a.head_dim = 1, 96

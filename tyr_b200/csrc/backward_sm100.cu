@@ -84,7 +84,10 @@ struct BCfg {
   static constexpr int dp_full = kB + 11;              // dP^T in tensor memory
   static constexpr int dp_taken = kB + 12;             // dP^T is in registers: its columns are free (8 warp arrivals)
   static constexpr int p_half = kB + 13;               // kHalfP: P^T of query columns 0..63 written (8 warp arrivals)
-  static constexpr int kNumBars = kB + 14;
+  // units handed out by a counter (kSink): [2] each
+  static constexpr int unit_full = kB + 14;            // the number of the next unit is in shared memory
+  static constexpr int unit_empty = kB + 16;           // the issuer and the 8 elementwise warps have read it
+  static constexpr int kNumBars = kB + 18;
   // D = 128: P^T is handed over in two halves, so that dV of the first 64 query columns runs during the
   // exponentials of the second 64.  The backward of 4096 rows, 32/8 heads 396.7 -> 391.9 us, of 8 x 2048 rows,
   // 16/8 heads 480.3 -> 477.8, of 2304 rows x 24 heads without a mask 185.6 -> 183.4; at D = 64, where the elementwise warps are the bound, the extra hand-over cost 0.3 %.
@@ -121,6 +124,7 @@ struct BwdParams {
   // kSink only: the first n_sink keys are visible to every later row beside the window.  Their sink_blk key blocks are
   // done in sink_parts units each, whose partial dK and dV (fp32) go to sink_out and are added by bwd_sink_merge_kernel.
   int n_sink, sink_blk, sink_parts;
+  int* next_unit;        // units taken by the dK/dV kernel's CTAs beyond their first, zeroed by the row statistics kernel
   float* sink_out;       // [sink_blk][sink_parts][batch][n_kv_head][dK, dV][128 keys][D]; null when sink_parts is 1
 };
 
@@ -244,6 +248,11 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   const int n_units = kv_units<kSink>(p);
   const int n_rounds = kCluster ? 1 : rounds_of(n_units);
   const UnitPart part = {kCluster ? static_cast<int>(cluster_rank()) : 0, kCluster ? p.parts : 1};
+  // First tokens' units are not the last ones' length: the CTAs take the next unit as they come free, in the order of the
+  // units, longest first.  (Which CTA does a unit does not change its sums.)  2 x 4096 rows, 16/8 heads of 128, window
+  // 1024: the longest CTA had 68 pairs of 59.5 on average in mirrored rounds.
+  constexpr bool kCounted = kSink && !kCluster;
+  __shared__ int taken[2];
   auto unit_at = [&](int round) { return kCluster ? static_cast<int>(blockIdx.x) / part.size : unit_of_round(round, n_units); };
   auto unit = [&](int u) {
     KvUnit w = kv_unit<kSink>(u, p);
@@ -256,6 +265,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     wait_ctl.limit = p.wait_limit;
     for (int i = 0; i < C::kNumBars; ++i)
       mbar_init(bar(i), (i == C::p_half || i == C::p_full || i == C::ds_half || i == C::ds_full || i == C::dp_taken || i == C::acc_free) ? 8u
+                        : (i == C::unit_empty || i == C::unit_empty + 1) ? 9u
                         : (i >= C::pair && i < C::pair + 4) ? 2u : 1u);
     mbar_fence_init();
     tma_prefetch_desc(&tm_k);
@@ -283,13 +293,26 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   }
   __syncwarp();
 
+  // the unit of a round for the issuing and elementwise warps; -1: no more, or a wait gave up
+  auto counted_unit = [&](int round) {
+    if (round == 0) return static_cast<int>(blockIdx.x);
+    const int slot = (round - 1) & 1;
+    if (!__all_sync(0xffffffffu, mbar_wait_q(bar(C::unit_full + slot), ((round - 1) >> 1) & 1, abortp))) return -1;
+    const int u = taken[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(C::unit_empty + slot));
+    return u;
+  };
+
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       bool ok = true;
       int it = 0, rc = 0;
-      for (int round = 0; round < n_rounds && ok; ++round) {
-        const int u = unit_at(round);
+      int next = kCounted ? static_cast<int>(blockIdx.x) : 0;
+      for (int round = 0; (kCounted || round < n_rounds) && ok; ++round) {
+        const int u = kCounted ? next : unit_at(round);
+        if (kCounted && u < 0) break;
         if (u < 0) continue;
         const KvUnit w = unit(u);
         if (w.n_iter == 0) continue;
@@ -301,12 +324,18 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
           tma_load_4d(base + C::kRes1 + kb * C::kBoxBytes, &tm_k, bar(C::res_full), kb * 64, w.blk * kT, w.head, w.b);
           tma_load_4d(base + C::kRes2 + kb * C::kBoxBytes, &tm_v, bar(C::res_full), kb * 64, w.blk * kT, w.head, w.b);
         }
+        int head_at = kCounted ? w.first / w.per_head : 0, blk_at = kCounted ? w.first % w.per_head : 0;
         for (int i = 0; i < w.n_iter && ok; ++i, ++it) {
           const int s = it % C::kStages;
           if (it >= C::kStages) ok = mbar_wait_q(bar(C::str_empty + s), ((it / C::kStages) - 1) & 1, abortp);
           if (!ok) break;
-          const int gi = kCluster ? part.pair(i) : kSink ? w.first + i : i;
-          const int hq = w.head * p.group + gi / w.per_head, qblk = w.lo + gi % w.per_head;
+          const int gi = kCluster ? part.pair(i) : i;
+          const int hq = w.head * p.group + (kCounted ? head_at : gi / w.per_head);
+          const int qblk = w.lo + (kCounted ? blk_at : gi % w.per_head);
+          if (kCounted && ++blk_at == w.per_head) {
+            blk_at = 0;
+            ++head_at;
+          }
           const uint32_t dst = base + C::kStr + s * 2 * C::kTileBytes;
           mbar_expect_tx(bar(C::str_full + s), 2 * C::kTileBytes + C::kStatBytes);
           {
@@ -320,6 +349,16 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             tma_load_4d(dst + kb * C::kBoxBytes, &tm_q, bar(C::str_full + s), kb * 64, qblk * kT, hq, w.b);
             tma_load_4d(dst + C::kTileBytes + kb * C::kBoxBytes, &tm_do, bar(C::str_full + s), kb * 64, qblk * kT,
                         hq, w.b);
+          }
+          if (kCounted && i == 0) {
+            // (every unit has a pair.)  The next unit's number, behind this one's first loads
+            const int slot = round & 1;
+            next = static_cast<int>(gridDim.x) + atomicAdd(p.next_unit, 1);
+            if (next >= n_units) next = -1;
+            if (round >= 2) ok = mbar_wait_q(bar(C::unit_empty + slot), ((round >> 1) - 1) & 1, abortp);
+            if (!ok) break;
+            taken[slot] = next;
+            mbar_arrive(bar(C::unit_full + slot));
           }
         }
         ++rc;
@@ -357,8 +396,9 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       };
       bool ok = true;
       int it = 0, rc = 0;
-      for (int round = 0; round < n_rounds && ok; ++round) {
-        const int u = unit_at(round);
+      for (int round = 0; (kCounted || round < n_rounds) && ok; ++round) {
+        const int u = kCounted ? counted_unit(round) : unit_at(round);
+        if (kCounted && u < 0) break;
         if (u < 0) continue;
         const KvUnit w = unit(u);
         if (w.n_iter == 0) continue;
@@ -432,11 +472,13 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     const uint64_t sl2x2 = pack_f32x2(p.sl2, p.sl2), scale2 = pack_f32x2(p.scale, p.scale);
     bool ok = true;
     int it = 0, rc = 0;
-    for (int round = 0; round < n_rounds && ok; ++round) {
-      const int u = unit_at(round);
+    for (int round = 0; (kCounted || round < n_rounds) && ok; ++round) {
+      const int u = kCounted ? counted_unit(round) : unit_at(round);
+      if (kCounted && u < 0) break;
       if (u < 0) continue;
       const KvUnit w = unit(u);
       const int row0 = w.blk * kT;
+      int blk_at = kCounted ? w.first % w.per_head : 0;
       for (int i = 0; i < w.n_iter; ++i, ++it) {
         // the score regions swap roles with every streamed pair (see the MMA issuer)
         const uint32_t tS = tmem + lane_addr + ((it & 1) ? C::kTmemDP : C::kTmemS);
@@ -449,7 +491,8 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         if (!ok) break;
         tc_fence_after();
         // first query of the score columns
-        const int col0 = (w.lo + (kCluster ? part.pair(i) : kSink ? w.first + i : i) % w.per_head) * kT;
+        const int col0 = (w.lo + (kCounted ? blk_at : (kCluster ? part.pair(i) : i) % w.per_head)) * kT;
+        if (kCounted && ++blk_at == w.per_head) blk_at = 0;
         // under the causal mask a key row keeps the query columns with query >= key
         int c_first = p.causal ? row0 + r - col0 : 0;
         // sliding window: the key also drops out for queries with query - key >= window
@@ -467,7 +510,6 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         // and 1, which belong to different warps of the pair: the two meet once both hold their
         // columns in registers.  P stays in registers as fp32 for dS.
         uint32_t pr2[2][32];
-        uint32_t dead = 0;  // kSink: bit `step`: P and dS of this warp's chunk are zero
 #pragma unroll
         for (int step = 0; step < 2; ++step) tmem_ld32(tS + (2 * step + half) * 32, pr2[step]);
         tmem_wait_ld();
@@ -481,25 +523,16 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
           const int c = 2 * step + half;
           uint32_t(&sr)[32] = pr2[step];
           if (kSink && masked) {
-            // as bits; a chunk that no key row of the warp is seen by needs no exponentials
             const uint32_t bits = ~bits_below(c_first - 32 * c) & bits_below(c_limit - 32 * c);
-            if (__all_sync(0xffffffffu, bits == 0u)) {
-              dead |= 1u << step;
-            } else {
 #pragma unroll
-              for (int x = 0; x < 32; ++x)
-                if (!(bits & (1u << x))) sr[x] = 0xff800000u;  // -inf: P = 0
-            }
+            for (int x = 0; x < 32; ++x)
+              if (!(bits & (1u << x))) sr[x] = 0xff800000u;  // -inf: P = 0
           } else if (masked) {
 #pragma unroll
             for (int x = 0; x < 32; ++x)
               if (c * 32 + x < c_first || c * 32 + x >= c_limit) sr[x] = 0xff800000u;  // -inf: P = 0
           }
           uint32_t pk_p[16];
-          if (kSink && ((dead >> step) & 1u)) {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) pk_p[x] = 0u;
-          } else
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
             // statistics of the two query columns (every lane reads the same addresses)
@@ -554,10 +587,6 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
           uint32_t(&pr)[32] = pr2[step];
           uint32_t(&dp)[32] = dp2[step];
           uint32_t pk_s[16];
-          if (kSink && ((dead >> step) & 1u)) {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) pk_s[x] = 0u;
-          } else
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
             const float2 d = *reinterpret_cast<const float2*>(nd_col + c * 32 + 2 * x);
@@ -1100,10 +1129,11 @@ __global__ void __launch_bounds__(256)
 bwd_rowstats_kernel(const __nv_bfloat16* o, const __nv_bfloat16* d_o, const float* lse, float* neg_lse2,
                     float* neg_delta_s, int n_head, int q_seq, int sq_pad, int64_t os_b,
                     int64_t os_h, int64_t os_s, int64_t ds_b, int64_t ds_h, int64_t ds_s, float scale,
-                    int64_t total_rows) {
+                    int64_t total_rows, int* next_unit) {
   constexpr int kLanes = D / 8;  // lanes per row
   grid_launch_dependents();      // the dK/dV kernel may set up; it waits for this grid itself
   grid_dependency_wait();
+  if (next_unit != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *next_unit = 0;
   const int64_t slot = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / kLanes;  // padded row index
   const int sub = threadIdx.x % kLanes;
   if (slot >= total_rows) return;
@@ -1196,6 +1226,8 @@ SinkPlan sink_plan(const TyrAttnBackwardArgs& a, int n_sink, int sms) {
   if (s.parts > 1) s.bytes = (size_t)s.blk * s.parts * a.batch * a.n_kv_head * 2 * kT * a.head_dim * sizeof(float);
   return s;
 }
+constexpr size_t kCounterBytes = 256;
+// behind the row statistics: the counter of the units, then the parts' sums
 size_t sink_parts_offset(const TyrAttnBackwardArgs& a) {
   return (backward_workspace_bytes(a.batch, a.n_head, a.q_seq) + 255) & ~(size_t)255;
 }
@@ -1208,6 +1240,7 @@ int launch_bwd(const TyrAttnBackwardArgs& a, int n_sink, float scale, int* statu
   const int64_t padded_rows = (int64_t)a.batch * a.n_head * sq_pad;
   float* neg_lse2 = static_cast<float*>(a.workspace);
   float* neg_delta_s = neg_lse2 + padded_rows;
+  int* next_unit = kSink ? reinterpret_cast<int*>(static_cast<char*>(a.workspace) + sink_parts_offset(a)) : nullptr;
 
   CUtensorMap tq, tk, tv, tdo;
   int rc;
@@ -1240,7 +1273,7 @@ int launch_bwd(const TyrAttnBackwardArgs& a, int n_sink, float scale, int* statu
         bwd_rowstats_kernel<D>, dim3((unsigned)blocks), dim3(256), 0, st, 1,
         static_cast<const __nv_bfloat16*>(a.o), static_cast<const __nv_bfloat16*>(a.d_o), a.lse, neg_lse2,
         neg_delta_s, a.n_head, a.q_seq, sq_pad, a.o_stride[0], a.o_stride[1], a.o_stride[2], a.do_stride[0],
-        a.do_stride[1], a.do_stride[2], scale, padded_rows);
+        a.do_stride[1], a.do_stride[2], scale, padded_rows, next_unit);
     count_launch();
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) return (int)e;
@@ -1284,10 +1317,11 @@ int launch_bwd(const TyrAttnBackwardArgs& a, int n_sink, float scale, int* statu
   p.sink_blk = sink.blk;
   p.sink_parts = 1;
   p.sink_out = nullptr;
+  p.next_unit = next_unit;
   p.parts = unit_parts<D, kSink>(p, dev, sms);
   if (kSink && p.parts == 1 && sink.parts > 1) {  // (the CTAs of a cluster share a long unit by themselves)
     p.sink_parts = sink.parts;
-    p.sink_out = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + sink_parts_offset(a));
+    p.sink_out = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + sink_parts_offset(a) + kCounterBytes);
   }
   const long long units_kv = p.sink_parts > 1 ? grid_kv : (long long)n_kblk * a.n_kv_head * a.batch;
   cudaError_t e = p.parts > 1
@@ -1338,7 +1372,7 @@ size_t backward_workspace_bytes(int batch, int n_head, int q_seq) {
 
 size_t backward_sinks_workspace_bytes(const TyrAttnBackwardArgs& a, int n_sink) {
   const SinkPlan s = sink_plan(a, n_sink, sms_of_device());
-  return s.bytes ? sink_parts_offset(a) + s.bytes : backward_workspace_bytes(a.batch, a.n_head, a.q_seq);
+  return sink_parts_offset(a) + kCounterBytes + s.bytes;
 }
 
 int launch_backward_sm100(const TyrAttnBackwardArgs& a, int n_sink, float scale, int* status, cudaStream_t st) {

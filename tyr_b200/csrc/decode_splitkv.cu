@@ -78,7 +78,6 @@ struct PagedParams : DecodeParams {
   int64_t table_stride;
   FastDiv by_page;
   int n_pages, max_len, window, n_sink;
-  int one_layout;     // K and V have the same strides
   float* ws_scores;   // [batch, n_head, max_kv_seq] scores in the log2 domain, for the running sums of the weights; or null
 };
 template <class P>
@@ -217,22 +216,32 @@ decode_kernel(const __grid_constant__ P p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int quad = lane >> 2, t4 = lane & 3;
 
-  // ---- paged cache: where the rows of a tile lie.  The kLoads rows a thread loads a piece of are the same for the
-  // kChunksPerRow lanes of its group, so each lane looks one of them up, a tile ahead of the loads, and the lanes exchange
-  // the offsets: neither a table entry's latency (nothing looks at it before the loads need it) nor a 64-bit
-  // product for every piece is on the path of the loads.
-  constexpr int kLoads = kTileKeys * C::kChunksPerRow / kThreads, kRowStep = kThreads / C::kChunksPerRow;
+  // ---- paged cache: where the rows of a tile lie.  A thread loads a piece of kLoads rows, one below the other, as do the other
+  // lanes of its group of kChunksPerRow, so each lane finds the place of one of them.  The page table's entries come
+  // through shared memory, one per row, fetched with the rows of the tile two before: a register that waits for
+  // memory would hold up the loop (a table entry in a register a tile ahead cost 11 us of 87 at pages of 16 rows).
+  constexpr int kLoads = kTileKeys * C::kChunksPerRow / kThreads;
+  constexpr int kEntrySlots = 4;
+  __shared__ int entries[kPaged ? kEntrySlots * kTileKeys : 1];
   struct Where { int page, row; };
   bool bad_page = false;
-  auto look_up = [&](int tile) {
+  auto key_of = [&](int tile, int kr) {  // key of the sequence in row kr of the tile
+    const int v = min(key_begin + tile * kTileKeys + kr, key_end - 1);
+    return v + (v >= vis.first ? vis.gap : 0);
+  };
+  auto fetch_entries = [&](int tile) {
+    if constexpr (kPaged) {
+      if (tile < n_tiles && tid < kTileKeys)
+        cp_async4(smem_u32(&entries[tile % kEntrySlots * kTileKeys + tid]), p.table + b * p.table_stride + p.by_page.div(key_of(tile, tid)));
+    }
+  };
+  auto look_up = [&](int tile, bool direct) {
     Where w{0, 0};
     if constexpr (kPaged) {
-      const int kr = (lane % C::kChunksPerRow) % kLoads * kRowStep + tid / C::kChunksPerRow;
-      const int v = min(key_begin + tile * kTileKeys + kr, key_end - 1);
-      const int key = v + (v >= vis.first ? vis.gap : 0);
-      const int at = p.by_page.div(key);
+      const int kr = tid / C::kChunksPerRow * kLoads + lane % C::kChunksPerRow % kLoads;
+      const int key = key_of(tile, kr), at = p.by_page.div(key);
       w.row = key - at * (int)p.by_page.d;
-      w.page = p.table[b * p.table_stride + at];
+      w.page = direct ? p.table[b * p.table_stride + at] : entries[tile % kEntrySlots * kTileKeys + kr];
     }
     return w;
   };
@@ -241,26 +250,35 @@ decode_kernel(const __grid_constant__ P p) {
   auto load_tile = [&](int tile, int stage, Where where) {
     const uint32_t sk = sbase + stage * C::kStageBytes, sv = sk + C::kTileBytes;
     const int k0 = key_begin + tile * kTileKeys;
-    long long at_k = 0, at_v = 0;
     if constexpr (kPaged) {
       if ((unsigned)where.page >= (unsigned)p.n_pages) {  // not followed
         bad_page = true;
         where.page = 0;
       }
-      at_k = where.page * p.ks[0] + where.row * p.ks[2];
-      at_v = p.one_layout ? at_k : where.page * p.vs[0] + where.row * p.vs[2];
+      const int c = tid % C::kChunksPerRow, kr0 = tid / C::kChunksPerRow * kLoads, mine = c % kLoads;
+      const long long at_k = where.page * p.ks[0] + where.row * p.ks[2], at_v = where.page * p.vs[0] + where.row * p.vs[2];
+      const long long k0_at = __shfl_sync(0xffffffffu, at_k, 0, C::kChunksPerRow), v0_at = __shfl_sync(0xffffffffu, at_v, 0, C::kChunksPerRow);
+      if (__all_sync(0xffffffffu, at_k == k0_at + mine * p.ks[2] && at_v == v0_at + mine * p.vs[2])) {
+        // the usual case: a thread's rows lie in one page
+        const __nv_bfloat16 *kp = kbase + c * 8 + k0_at, *vp = vbase + c * 8 + v0_at;
+#pragma unroll
+        for (int it = 0; it < kLoads; ++it, kp += p.ks[2], vp += p.vs[2]) {
+          cp_async16(sk + sw_off<D>(kr0 + it, c), kp);
+          cp_async16(sv + sw_off<D>(kr0 + it, c), vp);
+        }
+      } else {
+#pragma unroll
+        for (int it = 0; it < kLoads; ++it) {
+          cp_async16(sk + sw_off<D>(kr0 + it, c), kbase + c * 8 + __shfl_sync(0xffffffffu, at_k, it, C::kChunksPerRow));
+          cp_async16(sv + sw_off<D>(kr0 + it, c), vbase + c * 8 + __shfl_sync(0xffffffffu, at_v, it, C::kChunksPerRow));
+        }
+      }
+      return;
     }
 #pragma unroll
     for (int it = 0; it < kLoads; ++it) {
       const int idx = it * kThreads + tid;
       const int kr = idx / C::kChunksPerRow, c = idx % C::kChunksPerRow;
-      if constexpr (kPaged) {
-        const long long k_at = __shfl_sync(0xffffffffu, at_k, it, C::kChunksPerRow);
-        const long long v_at = p.one_layout ? k_at : __shfl_sync(0xffffffffu, at_v, it, C::kChunksPerRow);
-        cp_async16(sk + sw_off<D>(kr, c), kbase + c * 8 + k_at);
-        cp_async16(sv + sw_off<D>(kr, c), vbase + c * 8 + v_at);
-        continue;
-      }
       const int key = min(k0 + kr, key_end - 1);  // rows past the end re-read the last valid key
       cp_async16(sk + sw_off<D>(kr, c), kbase + (int64_t)key * p.ks[2] + c * 8);
       cp_async16(sv + sw_off<D>(kr, c), vbase + (int64_t)key * p.vs[2] + c * 8);
@@ -271,16 +289,13 @@ decode_kernel(const __grid_constant__ P p) {
   if constexpr (kPaged) {
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s)
-      if (s < n_tiles) ahead[s] = look_up(s);
+      if (s < n_tiles) ahead[s] = look_up(s, true);
   }
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
     if (s < n_tiles) load_tile(s, s, ahead[s]);
+    fetch_entries(s + kStages - 1);
     cp_async_commit();
-  }
-  Where next{0, 0};
-  if constexpr (kPaged) {
-    if (kStages - 1 < n_tiles) next = look_up(kStages - 1);
   }
 
   // ---- Q fragments (B operand: column = query row of this KV head)
@@ -312,11 +327,11 @@ decode_kernel(const __grid_constant__ P p) {
   for (int tile = 0; tile < n_tiles; ++tile) {
     cp_async_wait<kStages - 2>();
     __syncthreads();
-    if (tile + kStages - 1 < n_tiles) load_tile(tile + kStages - 1, (tile + kStages - 1) % kStages, next);
+    // (the entries of the tile to load came with the rows of this one)
+    if (tile + kStages - 1 < n_tiles)
+      load_tile(tile + kStages - 1, (tile + kStages - 1) % kStages, look_up(tile + kStages - 1, false));
+    fetch_entries(tile + 2 * (kStages - 1));
     cp_async_commit();
-    if constexpr (kPaged) {
-      if (tile + kStages < n_tiles) next = look_up(tile + kStages);
-    }
 
     const int stage = tile % kStages;
     const uint32_t sk = sbase + stage * C::kStageBytes, sv = sk + C::kTileBytes;
@@ -596,25 +611,42 @@ decode_merge_kernel(const P p) {
 
 // Running sums of the weights: weights[b, hkv, key] += sum over the group's heads of 2^(score - lse).  The scores are those
 // the split kernel left in the workspace: 4 bytes per key and query head, where forming them again would read the key's
-// 2 D bytes a second time.  One thread per visible key, the group's heads in order: no atomics.
-constexpr int kSumThreads = 256;
+// 2 D bytes a second time.  A visible key belongs to one thread, which
+// takes the group's heads in order: no atomics.
+constexpr int kSumThreads = 256, kSumKeys = 4;  // keys per thread, kSumThreads apart: their loads are in flight together
 __global__ void __launch_bounds__(kSumThreads)
 weight_sums_kernel(const PagedParams p, float* weights, int64_t stride_b, int64_t stride_h) {
   grid_launch_dependents();
   grid_dependency_wait();
   const int hkv = blockIdx.y, b = blockIdx.z;
   const Visible vis = visible_of(min(max(p.kv_lens[b], 0), p.max_len), p);
-  const int v = blockIdx.x * kSumThreads + threadIdx.x;
-  if (v >= vis.n) return;
-  float acc = 0.f;
-  for (int r = 0; r < p.rows; ++r) {
-    const int64_t at = lse_index(p, b, hkv, r);
-    const float lse = p.lse[at];
-    // (a row without any weight, every score -inf, gives none)
-    acc += lse == -INFINITY ? 0.f : ex2f(p.ws_scores[at * p.max_kv_seq + v] - lse * kLog2e);
+  const int v0 = blockIdx.x * (kSumThreads * kSumKeys) + threadIdx.x;
+  if (v0 >= vis.n) return;
+  float* w = weights + b * stride_b + hkv * stride_h;
+  const int64_t row0 = lse_index(p, b, hkv, 0);
+  float acc[kSumKeys], old[kSumKeys];
+#pragma unroll
+  for (int k = 0; k < kSumKeys; ++k) {
+    const int v = v0 + k * kSumThreads;
+    acc[k] = 0.f;
+    old[k] = v < vis.n ? w[v + (v >= vis.first ? vis.gap : 0)] : 0.f;
   }
-  float* w = weights + b * stride_b + hkv * stride_h + v + (v >= vis.first ? vis.gap : 0);
-  *w += acc;
+#pragma unroll 4
+  for (int r = 0; r < p.rows; ++r) {
+    const float lse = p.lse[row0 + r];
+    const float* score = p.ws_scores + (row0 + r) * p.max_kv_seq;
+#pragma unroll
+    for (int k = 0; k < kSumKeys; ++k) {
+      const int v = v0 + k * kSumThreads;
+      // (a row without any weight, every score -inf, gives none)
+      if (v < vis.n && lse != -INFINITY) acc[k] += ex2f(score[v] - lse * kLog2e);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kSumKeys; ++k) {
+    const int v = v0 + k * kSumThreads;
+    if (v < vis.n) w[v + (v >= vis.first ? vis.gap : 0)] = old[k] + acc[k];
+  }
 }
 
 // Two-way merge, natural-log LSE (the formula of RingAttn.lean:164-180).
@@ -828,7 +860,6 @@ int launch_paged_decode(const TyrAttnPagedDecodeArgs& a, float scale, int* statu
   p.max_len = a.max_kv_seq;
   p.window = a.window_size;
   p.n_sink = a.n_sink;
-  p.one_layout = a.k_stride[0] == a.v_stride[0] && a.k_stride[2] == a.v_stride[2];
   if ((long long)p.n_kv_head * p.row_groups > 65535) return -TYR_ATTN_ERR_TOO_LARGE;  // (the grid's y extent)
   char* ws = static_cast<char*>(a.workspace);
   p.ws_o = reinterpret_cast<float*>(ws);
@@ -849,7 +880,7 @@ int launch_paged_decode(const TyrAttnPagedDecodeArgs& a, float scale, int* statu
   if (s.needs_workspace()) p.ws_lse = p.ws_o + (size_t)a.batch * a.n_head * s.n_splits * a.head_dim;
   const int rc = a.head_dim == 128 ? launch_d<128>(p, s, st) : launch_d<64>(p, s, st);
   if (rc || !a.weights) return rc;
-  const cudaError_t e = launch_overlapped(weight_sums_kernel, dim3((p.max_kv_seq + kSumThreads - 1) / kSumThreads, a.n_kv_head, a.batch),
+  const cudaError_t e = launch_overlapped(weight_sums_kernel, dim3((p.max_kv_seq + kSumThreads * kSumKeys - 1) / (kSumThreads * kSumKeys), a.n_kv_head, a.batch),
                                           dim3(kSumThreads), 0, st, 1, p, a.weights, a.weights_stride[0], a.weights_stride[1]);
   count_launch();
   return (int)(e != cudaSuccess ? e : cudaGetLastError());

@@ -138,6 +138,10 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
       const int i = i0 + k * kSelectThreads + tid;
+      if (i0 + k * kSelectThreads >= n) {
+        if (lane == 0) counts[k * (kSelectThreads / 32) + warp] = 0u;
+        continue;
+      }
       const uint32_t u = ordered(x[k]);
       const bool candidate = i >= lo && i < hi;
       const bool over = i < lo || (i >= hi && i < n) || (candidate && u > T), equal = candidate && u == T;
@@ -169,6 +173,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
+      if (i0 + k * kSelectThreads >= n) break;
       const bool over = (over_bits >> k) & 1u, equal = (equal_bits >> k) & 1u;
       const uint32_t lower = (1u << lane) - 1u, c = counts[k * (kSelectThreads / 32) + warp];
       const uint32_t over_at = over_before + (c & 0xffffu) + __popc(__ballot_sync(0xffffffffu, over) & lower);
