@@ -260,7 +260,7 @@ typedef struct TyrAttnPageTable {
  * `weights`, when not NULL, is a running sum per (sequence, KV head, key): the call adds, for every visible key, the
  * softmax weights that the query heads of the group gave it; entries of other keys stay as they are.  No atomics: the
  * same bits each time.
- * At most two launches, three with `weights`. */
+ * At most two launches. */
 typedef struct TyrAttnPagedDecodeArgs {
   const void* q; /* [batch, n_head, head_dim] */
   void* o;       /* [batch, n_head, head_dim] */

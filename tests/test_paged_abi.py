@@ -53,12 +53,15 @@ def test_decode(built_lib, mem):
     assert call(head_dim=96) == -3 and call(head_dim=256) == -3
     assert call(max_kv_seq=65) == -11                                # more than four pages of 16 rows
     assert call(pages=table(p, page_size=1 << 30)) == -10            # rows past 32 bits
+    assert call(pages=table(p, max_pages=2, page_size=(1 << 30) - 1), max_kv_seq=(1 << 30) + 1) == -10
     assert call(batch=65536) == -10 and call(n_kv_head=65537, n_head=65537) == -10
     for bad in (dict(k=p + 8), dict(v=p + 2), dict(k_stride=[2048, 1024, 60]), dict(v_stride=[2047, 1024, 64]), dict(k_stride=[2048, 1024, 0]),
                 dict(q=p + 2), dict(q_stride=[255, 64]), dict(o=p + 1), dict(weights=p + 2, weights_stride=[128, 64])):
         assert call(**bad) == -4, bad
     assert call(weights=p, weights_stride=[128, 32]) == -2           # rows of two heads overlap
     assert call(weights=p, weights_stride=[32, 64]) == -2
+    assert call(weights=p, weights_stride=[64, 64]) == -2            # the second head of one sequence is the first of the next
+    assert call(weights=p, weights_stride=[64, 127]) == -2 and call(weights=p, weights_stride=[64, 128]) == -7   # heads outermost: fine
     assert call(weights=p, weights_stride=[128, 64]) == -7           # the scores' workspace is missing
     assert call(weights=p, weights_stride=[128, 64], workspace=p + 8, workspace_bytes=1 << 20) == -7
     assert call(weights=p, weights_stride=[128, 64], workspace=p, workspace_bytes=2 * 4 * 65 * 4 - 1) == -7
@@ -104,12 +107,14 @@ def test_evict(built_lib, mem):
     assert call(batch=0) == 0
     for bad in (dict(batch=-1), dict(n_kv_head=0), dict(max_kv_seq=0), dict(n_keep=0), dict(n_recent=-1), dict(n_sink=-1),
                 dict(n_recent=8), dict(n_recent=2 ** 31 - 1, n_sink=2 ** 31 - 1), dict(new_lens=p), dict(weights_stride=[128, 63]),
-                dict(weights_stride=[0, 64]), dict(pages=table(p, table_stride=0))):
+                dict(weights_stride=[0, 64]), dict(weights_stride=[64, 64]), dict(pages=table(p, table_stride=0)),
+                dict(k_stride=[0, 1024, 64]), dict(v_stride=[2048, 0, 64]), dict(k_stride=[2048, 1024, 56])):
         assert call(**bad) == -2, bad
     assert call(head_dim=96) == -3
     assert call(max_kv_seq=65, weights_stride=[256, 128]) == -11
     assert call(k=p + 8) == -4 and call(v_stride=[2048, 1024, 4]) == -4
     assert call(n_kv_head=70000) == -10
+    assert call(pages=table(p, max_pages=2, page_size=(1 << 30) - 1), max_kv_seq=(1 << 30) + 1) == -10
 
 
 def test_append(built_lib, mem):
@@ -121,7 +126,10 @@ def test_append(built_lib, mem):
         a.x_stride[:] = [3 * 2 * 64, 2 * 64, 64]
         a.out_stride[:] = [2 * 16 * 64, 16 * 64, 64]
         for k, v in kw.items():
-            setattr(a, k, v)
+            if isinstance(v, list):
+                getattr(a, k)[:] = v
+            else:
+                setattr(a, k, v)
         return f(ctypes.byref(a), ctypes.byref(pages if pages is not None else table(p)), None, None)
 
     assert f(None, ctypes.byref(table(p)), None, None) == -1 and call(pages=table(None)) == -1 and call(x=None) == -1
@@ -129,6 +137,7 @@ def test_append(built_lib, mem):
     assert call(position0=62) == -11                                 # rows 62..64 of 64
     assert call(pages=table(p, page_size=1 << 29)) == -10
     assert call(out=p + 8) == -4 and call(head_dim=96) == -3
+    assert call(out_stride=[2048, 0, 64]) == -2 and call(out_stride=[0, 1024, 64]) == -2      # heads or pages on one another
     assert call(cos=p, sin=p) == -2                                  # a rotary table without rows
     assert call(cos=p, sin=p, max_pos=2) == -11
 

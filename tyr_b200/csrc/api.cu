@@ -147,10 +147,18 @@ int check_page_table(const TyrAttnPageTable& t, int64_t max_kv_seq) {
 bool pool_aligned(const void* pool, const int64_t* stride) {
   return aligned16(pool) && !((stride[0] | stride[1] | stride[2]) & 7) && stride[2] > 0 && stride[0] >= 0 && stride[1] >= 0;
 }
+// a pool that is written to: no two of its rows overlap along any axis
+bool pool_rows_apart(const int64_t* stride, int n_pages, int heads, int page_size, int head_dim) {
+  return (n_pages == 1 || stride[0] >= head_dim) && (heads == 1 || stride[1] >= head_dim) && (page_size == 1 || stride[2] >= head_dim);
+}
 // the (sequence, KV head) rows of the running sums are written by different CTAs: they may not overlap
-bool sums_apart(const int64_t* stride, int batch, int n_kv_head, int max_kv_seq) {
+bool sums_apart(const int64_t* stride, int64_t batch, int64_t n_kv_head, int64_t max_kv_seq) {
+  if (batch > 1 && n_kv_head > 1)
+    return std::min(stride[0], stride[1]) >= max_kv_seq &&
+           (stride[0] >= (n_kv_head - 1) * stride[1] + max_kv_seq || stride[1] >= (batch - 1) * stride[0] + max_kv_seq);
   return (batch == 1 || stride[0] >= max_kv_seq) && (n_kv_head == 1 || stride[1] >= max_kv_seq);
 }
+constexpr int kMaxPagedKeys = 1 << 30;  // of a sequence, visible (the cut into chunks adds a chunk to it in 32 bits)
 int check_paged_decode_sizes(const TyrAttnPagedDecodeArgs* a) {
   if (!a) return -TYR_ATTN_ERR_NULL;
   if (a->batch <= 0 || a->n_head <= 0 || a->n_kv_head <= 0 || a->max_kv_seq <= 0) return -TYR_ATTN_ERR_SHAPE;
@@ -158,6 +166,7 @@ int check_paged_decode_sizes(const TyrAttnPagedDecodeArgs* a) {
   if (a->window_size < 0 || a->n_sink < 0 || (a->n_sink > 0 && a->window_size == 0)) return -TYR_ATTN_ERR_SHAPE;
   if (a->head_dim != 64 && a->head_dim != 128) return -TYR_ATTN_ERR_HEAD_DIM;
   if (a->batch > 65535 || a->n_kv_head > 65535) return -TYR_ATTN_ERR_TOO_LARGE;
+  if (a->max_kv_seq > kMaxPagedKeys && (a->window_size == 0 || (int64_t)a->window_size + a->n_sink > kMaxPagedKeys)) return -TYR_ATTN_ERR_TOO_LARGE;
   return 0;
 }
 
@@ -353,13 +362,16 @@ int tyr_b200_attn_paged_evict(const TyrAttnEvictArgs* a, void* stream) {
   if (a->batch <= 0 || a->n_kv_head <= 0 || a->max_kv_seq <= 0) return -TYR_ATTN_ERR_SHAPE;
   if (a->n_keep <= 0 || a->n_recent < 0 || a->n_sink < 0 || (int64_t)a->n_recent + a->n_sink > a->n_keep) return -TYR_ATTN_ERR_SHAPE;
   if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return -TYR_ATTN_ERR_HEAD_DIM;
-  if (a->batch > 65535 || a->n_kv_head > 65535) return -TYR_ATTN_ERR_TOO_LARGE;
+  if (a->batch > 65535 || a->n_kv_head > 65535 || a->max_kv_seq > kMaxPagedKeys) return -TYR_ATTN_ERR_TOO_LARGE;
   if (!sums_apart(a->weights_stride, a->batch, a->n_kv_head, a->max_kv_seq)) return -TYR_ATTN_ERR_SHAPE;
   if (a->batch > 1 && a->pages.table_stride == 0) return -TYR_ATTN_ERR_SHAPE;  // one row of the table for all: shared pages
   if (a->new_lens == a->kv_lens) return -TYR_ATTN_ERR_SHAPE;  // the lengths are read until the last row has moved
   int rc = check_page_table(a->pages, a->max_kv_seq);
   if (rc) return rc;
   if (!pool_aligned(a->k, a->k_stride) || !pool_aligned(a->v, a->v_stride)) return -TYR_ATTN_ERR_ALIGN;
+  for (const int64_t* st : {a->k_stride, a->v_stride})
+    if (!pool_rows_apart(st, a->pages.n_pages, a->n_kv_head, a->pages.page_size, a->head_dim)) return -TYR_ATTN_ERR_SHAPE;
+  if (reinterpret_cast<uintptr_t>(a->weights) & 3u) return -TYR_ATTN_ERR_ALIGN;
   int dev = 0;
   if ((rc = current_device_checked(&dev))) return rc;
   DeviceState* ds = device_state(dev);
@@ -387,7 +399,7 @@ static int qk_prologue(const TyrAttnPrologueArgs* a, const TyrAttnPageTable* pag
   if (pages) {
     const int rc = check_page_table(*pages, 0);
     if (rc) return rc;
-    if (a->out_at_row0) return -TYR_ATTN_ERR_SHAPE;
+    if (a->out_at_row0 || !pool_rows_apart(a->out_stride, pages->n_pages, a->n_head, pages->page_size, a->head_dim)) return -TYR_ATTN_ERR_SHAPE;
     cap = (int64_t)pages->max_pages * pages->page_size;
   }
   if (cap <= 0 || ((a->cos || a->pe) && a->max_pos <= 0)) return -TYR_ATTN_ERR_SHAPE;

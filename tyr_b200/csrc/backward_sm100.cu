@@ -185,11 +185,13 @@ struct KvUnit {
   int first;     // kSink: the unit's first streamed pair of the block's, and which of its parts it is
   int part;
 };
-template <bool kSink>
+// First tokens that stay visible beside a window (BwdParams): none; some; some, with their key blocks done in parts.
+constexpr int kNoSink = 0, kSinkWhole = 1, kSinkParts = 2;
+template <int kSink>
 __device__ __forceinline__ int kv_units(const BwdParams& p) {
-  return (p.n_kblk + (kSink ? p.sink_blk * (p.sink_parts - 1) : 0)) * p.n_kv_head * p.batch;
+  return (p.n_kblk + (kSink == kSinkParts ? p.sink_blk * (p.sink_parts - 1) : 0)) * p.n_kv_head * p.batch;
 }
-template <bool kSink>
+template <int kSink>
 __device__ __forceinline__ KvUnit kv_unit(int u, const BwdParams& p) {
   KvUnit w;
   w.first = w.part = 0;
@@ -198,17 +200,17 @@ __device__ __forceinline__ KvUnit kv_unit(int u, const BwdParams& p) {
   w.head = rem % p.n_kv_head;
   w.b = rem / p.n_kv_head;
   w.blk = lvl;
-  const int in_parts = kSink ? p.sink_blk * p.sink_parts : 0;  // units per head of the blocks of first tokens
-  if (kSink) {
+  const int in_parts = kSink == kSinkParts ? p.sink_blk * p.sink_parts : 0;  // units per head of the blocks of first tokens
+  if (kSink == kSinkParts) {
     w.blk = lvl < in_parts ? lvl / p.sink_parts : lvl - in_parts + p.sink_blk;
     w.part = lvl < in_parts ? lvl % p.sink_parts : 0;
   }
   w.lo = p.causal ? min(w.blk, p.n_qblk) : 0;
   int hi = p.n_qblk;  // one past the last query block that sees a key of the unit
-  if (p.window > 0 && !(kSink && w.blk < p.sink_blk)) hi = min(hi, (w.blk * kT + kT - 1 + p.window - 1) / kT + 1);
+  if (p.window > 0 && !(kSink != kNoSink && w.blk < p.sink_blk)) hi = min(hi, (w.blk * kT + kT - 1 + p.window - 1) / kT + 1);
   w.per_head = max(hi - w.lo, 0);
   w.n_iter = w.per_head * p.group;
-  if (kSink && lvl < in_parts) {
+  if (kSink == kSinkParts && lvl < in_parts) {
     const int n = w.n_iter;
     w.first = (int)((long long)n * w.part / p.sink_parts);
     w.n_iter = (int)((long long)n * (w.part + 1) / p.sink_parts) - w.first;
@@ -229,8 +231,7 @@ struct UnitPart {
 // tiles of the unit stay in shared memory (the next unit's are fetched as soon as the unit's last
 // score products have read them), Q and dO stream.  Barrier phases run on across units: every role
 // counts streamed tile pairs (`it`) and units with work (`rc`) for itself.
-// kSink: first tokens that stay visible beside a window (BwdParams).
-template <int D, bool kCluster, bool kSink>
+template <int D, bool kCluster, int kSink>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                 const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
@@ -248,10 +249,11 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
   const int n_units = kv_units<kSink>(p);
   const int n_rounds = kCluster ? 1 : rounds_of(n_units);
   const UnitPart part = {kCluster ? static_cast<int>(cluster_rank()) : 0, kCluster ? p.parts : 1};
-  // First tokens' units are not the last ones' length: the CTAs take the next unit as they come free, in the order of the
-  // units, longest first.  (Which CTA does a unit does not change its sums.)  2 x 4096 rows, 16/8 heads of 128, window
-  // 1024: the longest CTA had 68 pairs of 59.5 on average in mirrored rounds.
-  constexpr bool kCounted = kSink && !kCluster;
+  // With parts the units are of several lengths in no simple order: the CTAs take the next unit as they come free.  (Which
+  // CTA does a unit does not change its sums.)  2 x 4096 rows, 16/8 heads of 128, window 1024: in mirrored rounds the
+  // longest CTA has 68 pairs of 59.5 on average, this kernel 158 us against 153.  Units of a pair or two would feel
+  // the counter (64 x 6 heads of 256 rows x 64, not in parts: 31.2 us in rounds, 33.1 counted).
+  constexpr bool kCounted = kSink == kSinkParts && !kCluster;
   __shared__ int taken[2];
   auto unit_at = [&](int round) { return kCluster ? static_cast<int>(blockIdx.x) / part.size : unit_of_round(round, n_units); };
   auto unit = [&](int u) {
@@ -496,7 +498,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         // under the causal mask a key row keeps the query columns with query >= key
         int c_first = p.causal ? row0 + r - col0 : 0;
         // sliding window: the key also drops out for queries with query - key >= window
-        const int c_limit = p.window > 0 && !(kSink && row0 + r < p.n_sink) ? row0 + r - col0 + p.window : kT;
+        const int c_limit = p.window > 0 && !(kSink != kNoSink && row0 + r < p.n_sink) ? row0 + r - col0 + p.window : kT;
         // a padding key sees no query at all
         if (p.key_mask != nullptr && (row0 + r >= p.kv_seq || p.key_mask[w.b * p.key_mask_stride + row0 + r] == 0))
           c_first = kT;
@@ -522,7 +524,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         for (int step = 0; step < 2; ++step) {
           const int c = 2 * step + half;
           uint32_t(&sr)[32] = pr2[step];
-          if (kSink && masked) {
+          if (kSink != kNoSink && masked) {
             const uint32_t bits = ~bits_below(c_first - 32 * c) & bits_below(c_limit - 32 * c);
 #pragma unroll
             for (int x = 0; x < 32; ++x)
@@ -637,7 +639,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
       }
       const int row = row0 + r;
       const bool row_ok = row < p.kv_seq;
-      if (kSink && w.blk < p.sink_blk && p.sink_parts > 1) {
+      if (kSink == kSinkParts && w.blk < p.sink_blk) {
         float* out = p.sink_out + ((((int64_t)w.blk * p.sink_parts + w.part) * p.batch + w.b) * p.n_kv_head + w.head) * (2 * kT * D);
 #pragma unroll
         for (int which = 0; which < 2; ++which)
@@ -1184,7 +1186,7 @@ int unit_parts(const BwdParams& p, int dev, int sms) {
       cfg.attrs = &attr;
       cfg.numAttrs = 1;
       int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, bwd_dkdv_kernel<D, true, kSink>, &cfg) != cudaSuccess) {
+      if (cudaOccupancyMaxActiveClusters(&n, bwd_dkdv_kernel<D, true, kSink ? kSinkWhole : kNoSink>, &cfg) != cudaSuccess) {
         cudaGetLastError();  // no clusters of this size then
         n = 0;
       }
@@ -1235,6 +1237,7 @@ size_t sink_parts_offset(const TyrAttnBackwardArgs& a) {
 template <int D, bool kSink>
 int launch_bwd(const TyrAttnBackwardArgs& a, int n_sink, float scale, int* status, cudaStream_t st) {
   using C = BCfg<D>;
+  constexpr int kWhole = kSink ? kSinkWhole : kNoSink;
   const int n_qblk = (a.q_seq + kT - 1) / kT, n_kblk = (a.kv_seq + kT - 1) / kT;
   const int sq_pad = n_qblk * kT;
   const int64_t padded_rows = (int64_t)a.batch * a.n_head * sq_pad;
@@ -1253,10 +1256,12 @@ int launch_bwd(const TyrAttnBackwardArgs& a, int n_sink, float scale, int* statu
     static std::atomic<bool> attr_set[64] = {};
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -TYR_ATTN_ERR_NO_DEVICE;
     if (!attr_set[dev].load(std::memory_order_acquire)) {
-      cudaError_t e = cudaFuncSetAttribute(bwd_dkdv_kernel<D, false, kSink>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      cudaError_t e = cudaFuncSetAttribute(bwd_dkdv_kernel<D, false, kWhole>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            (int)C::kSmemBytes);
       if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(bwd_dkdv_kernel<D, true, kSink>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmemBytes);
+        e = cudaFuncSetAttribute(bwd_dkdv_kernel<D, true, kWhole>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmemBytes);
+      if (kSink && e == cudaSuccess)
+        e = cudaFuncSetAttribute(bwd_dkdv_kernel<D, false, kSinkParts>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmemBytes);
       if (e == cudaSuccess)
         e = cudaFuncSetAttribute(bwd_dq_kernel<D, kSink>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)DqCfg<D>::kSmemBytes);
@@ -1324,11 +1329,10 @@ int launch_bwd(const TyrAttnBackwardArgs& a, int n_sink, float scale, int* statu
     p.sink_out = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + sink_parts_offset(a) + kCounterBytes);
   }
   const long long units_kv = p.sink_parts > 1 ? grid_kv : (long long)n_kblk * a.n_kv_head * a.batch;
-  cudaError_t e = p.parts > 1
-                      ? launch_overlapped(bwd_dkdv_kernel<D, true, kSink>, dim3((unsigned)(units_kv * p.parts)), dim3(kBwdThreads),
-                                          C::kSmemBytes, st, (unsigned)p.parts, tk, tv, tq, tdo, p)
-                      : launch_overlapped(bwd_dkdv_kernel<D, false, kSink>, dim3((unsigned)std::min<long long>(units_kv, sms)),
-                                          dim3(kBwdThreads), C::kSmemBytes, st, 1, tk, tv, tq, tdo, p);
+  const dim3 units((unsigned)(p.parts > 1 ? units_kv * p.parts : std::min<long long>(units_kv, sms)));
+  auto* keys = p.parts > 1 ? bwd_dkdv_kernel<D, true, kWhole>
+               : p.sink_parts > 1 ? bwd_dkdv_kernel<D, false, kSink ? kSinkParts : kNoSink> : bwd_dkdv_kernel<D, false, kWhole>;
+  cudaError_t e = launch_overlapped(keys, units, dim3(kBwdThreads), C::kSmemBytes, st, (unsigned)p.parts, tk, tv, tq, tdo, p);
   count_launch();
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;

@@ -550,14 +550,10 @@ decode_kernel(const __grid_constant__ P p) {
 // kernel is still draining, and wait here until that grid has completed and its writes are visible,
 // so the launch latency of this second kernel hides behind the tail of the first.
 template <int D, class P>
-__global__ void __launch_bounds__(kMergeThreads)
-decode_merge_kernel(const P p) {
+__device__ __forceinline__ void merge_row(const P& p, int row, int b) {  // row of the sequence: head * q_seq + query
   constexpr int kLanes = D / 4, kGroups = kMergeThreads / kLanes;
   __shared__ float4 s_acc[kGroups][kLanes];
   __shared__ float s_w[kGroups];
-  grid_launch_dependents();
-  grid_dependency_wait();
-  const int row = blockIdx.x, b = blockIdx.y;  // row of the sequence: head * q_seq + query
   int len;
   if constexpr (kIsPaged<P>) len = visible_of(min(max(p.kv_lens[b], 0), p.max_len), p).n;
   else len = p.kv_lens ? min(max(p.kv_lens[b], 0), p.max_kv_seq) : p.max_kv_seq;
@@ -609,42 +605,84 @@ decode_merge_kernel(const P p) {
   }
 }
 
-// Running sums of the weights: weights[b, hkv, key] += sum over the group's heads of 2^(score - lse).  The scores are those
-// the split kernel left in the workspace: 4 bytes per key and query head, where forming them again would read the key's
-// 2 D bytes a second time.  A visible key belongs to one thread, which
-// takes the group's heads in order: no atomics.
-constexpr int kSumThreads = 256, kSumKeys = 4;  // keys per thread, kSumThreads apart: their loads are in flight together
-__global__ void __launch_bounds__(kSumThreads)
-weight_sums_kernel(const PagedParams p, float* weights, int64_t stride_b, int64_t stride_h) {
+template <int D, class P>
+__global__ void __launch_bounds__(kMergeThreads)
+decode_merge_kernel(const P p) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  merge_row<D>(p, blockIdx.x, blockIdx.y);
+}
+
+// The merge and, in the same launch, the running sums of the weights: weights[b, hkv, key] += sum over the group's heads of
+// 2^(score - lse).  The scores are those the split kernel left in the workspace: 4 bytes per key and query head, where
+// forming them again would read the key's 2 D bytes a second time.  A visible key belongs to one thread, which takes
+// the group's heads in order: no atomics.  The sums' CTAs find the rows' LSEs from the chunks' themselves, so they
+// wait for no merge (as a third launch behind it: 82 us instead of 79 on 16 sequences of 4096 to 8192 keys).
+constexpr int kSumKeys = 4;     // keys per thread, kMergeThreads apart: their loads are in flight together
+constexpr int kSumRows = 16;    // rows whose LSEs are held at a time
+template <int D>
+__global__ void __launch_bounds__(kMergeThreads)
+merge_and_sum_kernel(const PagedParams p, float* weights, int64_t stride_b, int64_t stride_h) {
   grid_launch_dependents();
   grid_dependency_wait();
   const int hkv = blockIdx.y, b = blockIdx.z;
+  if ((int)blockIdx.x < p.rows) {
+    if (p.ws_lse != nullptr) merge_row<D>(p, hkv * p.rows + blockIdx.x, b);
+    return;
+  }
+  __shared__ float s_lse[kSumRows];  // log2 domain
   const Visible vis = visible_of(min(max(p.kv_lens[b], 0), p.max_len), p);
-  const int v0 = blockIdx.x * (kSumThreads * kSumKeys) + threadIdx.x;
-  if (v0 >= vis.n) return;
+  const int first = (blockIdx.x - p.rows) * (kMergeThreads * kSumKeys), v0 = first + threadIdx.x;
+  if (first >= vis.n) return;
+  const int n_chunks = p.ws_lse != nullptr ? (vis.n + p.chunk_len - 1) / p.chunk_len : 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float* w = weights + b * stride_b + hkv * stride_h;
   const int64_t row0 = lse_index(p, b, hkv, 0);
   float acc[kSumKeys], old[kSumKeys];
 #pragma unroll
   for (int k = 0; k < kSumKeys; ++k) {
-    const int v = v0 + k * kSumThreads;
+    const int v = v0 + k * kMergeThreads;
     acc[k] = 0.f;
     old[k] = v < vis.n ? w[v + (v >= vis.first ? vis.gap : 0)] : 0.f;
   }
-#pragma unroll 4
-  for (int r = 0; r < p.rows; ++r) {
-    const float lse = p.lse[row0 + r];
-    const float* score = p.ws_scores + (row0 + r) * p.max_kv_seq;
+  for (int r0 = 0; r0 < p.rows; r0 += kSumRows) {
+    const int rows_here = min(kSumRows, p.rows - r0);
+    for (int r = warp; r < rows_here; r += kMergeThreads / 32) {
+      const int64_t row = row0 + r0 + r;
+      float lse;
+      if (n_chunks > 1) {  // at most 64 chunks: two per lane
+        const float* from = p.ws_lse + row * p.n_splits;
+        const float l0 = lane < n_chunks ? from[lane] : -INFINITY, l1 = lane + 32 < n_chunks ? from[lane + 32] : -INFINITY;
+        float M = fmaxf(l0, l1);
 #pragma unroll
-    for (int k = 0; k < kSumKeys; ++k) {
-      const int v = v0 + k * kSumThreads;
-      // (a row without any weight, every score -inf, gives none)
-      if (v < vis.n && lse != -INFINITY) acc[k] += ex2f(score[v] - lse * kLog2e);
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float ref = finite_ref(M);
+        float W = ex2f(l0 - ref) + ex2f(l1 - ref);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) W += __shfl_xor_sync(0xffffffffu, W, o);
+        lse = M + log2f(W);
+      } else {
+        lse = p.lse[row] * kLog2e;
+      }
+      if (lane == 0) s_lse[r] = lse;
     }
+    __syncthreads();
+#pragma unroll 4
+    for (int r = 0; r < rows_here; ++r) {
+      const float lse = s_lse[r];
+      const float* score = p.ws_scores + (row0 + r0 + r) * p.max_kv_seq;
+#pragma unroll
+      for (int k = 0; k < kSumKeys; ++k) {
+        const int v = v0 + k * kMergeThreads;
+        // (a row without any weight, every score -inf, gives none)
+        if (v < vis.n && lse != -INFINITY) acc[k] += ex2f(score[v] - lse);
+      }
+    }
+    __syncthreads();
   }
 #pragma unroll
   for (int k = 0; k < kSumKeys; ++k) {
-    const int v = v0 + k * kSumThreads;
+    const int v = v0 + k * kMergeThreads;
     if (v < vis.n) w[v + (v >= vis.first ? vis.gap : 0)] = old[k] + acc[k];
   }
 }
@@ -689,15 +727,16 @@ cudaError_t launch_scan_of(const P& p, const ScanPlan& s, cudaStream_t st) {
   return s.warps == 8 ? launch_scan<D, 8, kNT, false, P>(p, st) : launch_scan<D, 4, kNT, false, P>(p, st);
 }
 
+// `sums`: a paged call with running sums, whose merge comes with them.
 template <int D, class P>
-int launch_d(P& p, const ScanPlan& s, cudaStream_t st) {
+int launch_d(P& p, const ScanPlan& s, cudaStream_t st, bool sums = false) {
   if (!s.covers(p.max_kv_seq)) return -TYR_ATTN_ERR_SHAPE;  // (the kernel divides by the chunk length)
   p.n_splits = s.n_splits;
   p.chunk_len = s.chunk_len;
   cudaError_t e = p.rows <= 8 ? launch_scan_of<D, 1, P>(p, s, st) : launch_scan_of<D, 2, P>(p, s, st);
   count_launch();
   if (e != cudaSuccess) return (int)e;
-  if (s.needs_workspace()) {
+  if (s.needs_workspace() && !sums) {
     e = launch_overlapped(decode_merge_kernel<D, P>, dim3(p.n_head * p.q_seq, p.batch), dim3(kMergeThreads), 0, st, 1, p);
     count_launch();
   }
@@ -878,10 +917,13 @@ int launch_paged_decode(const TyrAttnPagedDecodeArgs& a, float scale, int* statu
                                      max_splits_of(a.max_splits), sm_count(), &pays);
   if (pays) s = own;
   if (s.needs_workspace()) p.ws_lse = p.ws_o + (size_t)a.batch * a.n_head * s.n_splits * a.head_dim;
-  const int rc = a.head_dim == 128 ? launch_d<128>(p, s, st) : launch_d<64>(p, s, st);
-  if (rc || !a.weights) return rc;
-  const cudaError_t e = launch_overlapped(weight_sums_kernel, dim3((p.max_kv_seq + kSumThreads * kSumKeys - 1) / (kSumThreads * kSumKeys), a.n_kv_head, a.batch),
-                                          dim3(kSumThreads), 0, st, 1, p, a.weights, a.weights_stride[0], a.weights_stride[1]);
+  const bool wide = a.head_dim == 128, sums = a.weights != nullptr;
+  const int rc = wide ? launch_d<128>(p, s, st, sums) : launch_d<64>(p, s, st, sums);
+  if (rc || !sums) return rc;
+  const int keys = kMergeThreads * kSumKeys;
+  const cudaError_t e = launch_overlapped(wide ? merge_and_sum_kernel<128> : merge_and_sum_kernel<64>,
+                                          dim3(p.rows + (p.max_kv_seq + keys - 1) / keys, a.n_kv_head, a.batch), dim3(kMergeThreads), 0, st,
+                                          1, p, a.weights, a.weights_stride[0], a.weights_stride[1]);
   count_launch();
   return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }

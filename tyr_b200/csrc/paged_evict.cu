@@ -47,7 +47,7 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 }
 
 // Positions a CTA holds at once, kItems of them per thread, position x * kSelectThreads + thread as item x.
-constexpr int kItems = 16, kSegment = kItems * kSelectThreads;
+constexpr int kItems = 16, kSegment = kItems * kSelectThreads, kAhead = 4;
 
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
   __shared__ uint32_t hist[256];
@@ -57,6 +57,15 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   grid_launch_dependents();
   grid_dependency_wait();
   const int hkv = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float* w = p.weights + b * p.w_stride_b + hkv * p.w_stride_h;
+  // a segment's weights stay in registers over all passes where there is only one; its first positions are fetched
+  // before the length is known (the array has max_len of them)
+  float x[kItems];
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int i = k * kSelectThreads + tid;
+    x[k] = k < kAhead && i < p.max_len ? w[i] : 0.f;
+  }
   const int raw = p.kv_lens[b], n = min(max(raw, 0), p.max_len);
   int32_t* kept = p.kept + ((int64_t)b * p.n_kv_head + hkv) * p.n_keep;
   if (hkv == 0 && tid == 0) {
@@ -67,20 +76,18 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     for (int i = tid; i < p.n_keep; i += kSelectThreads) kept[i] = i < n ? i : -1;
     return;
   }
-  float* w = p.weights + b * p.w_stride_b + hkv * p.w_stride_h;
   const int lo = p.n_sink, hi = n - p.n_recent;        // the candidates' positions
   const uint32_t m = p.n_keep - p.n_sink - p.n_recent;  // how many of them stay: fewer than there are
-  // a segment's weights stay in registers over all passes where there is only one
-  float x[kItems];
-  auto load = [&](int i0) {
+  auto load = [&](int i0, int k0) {
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
+      if (k < k0) continue;
       const int i = i0 + k * kSelectThreads + tid;
       x[k] = i < n ? w[i] : 0.f;
     }
   };
   const bool one_segment = n <= kSegment;
-  load(0);
+  load(0, kAhead);
   // T: the m-th greatest; `left`: how many of the keys equal to it stay
   uint32_t T = 0xffffffffu, left = 0;
   if (m > 0) {
@@ -91,7 +98,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
       __syncthreads();
       const uint32_t above = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
       for (int i0 = 0; i0 < hi; i0 += kSegment) {
-        if (!one_segment) load(i0);
+        if (!one_segment) load(i0, 0);
 #pragma unroll
         for (int k = 0; k < kItems; ++k) {
           const int i = i0 + k * kSelectThreads + tid;
@@ -133,7 +140,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   // in the order of the positions: a key stays if it always does, weighs more than T, or is one of the first `left` equal to T
   uint32_t over_before = 0, equal_before = 0;
   for (int i0 = 0; i0 < n; i0 += kSegment) {
-    if (!one_segment) load(i0);
+    if (!one_segment) load(i0, 0);
     uint32_t over_bits = 0, equal_bits = 0;  // of this thread's items
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
