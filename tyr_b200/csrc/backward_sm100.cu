@@ -520,16 +520,21 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::pair + quarter));
+        if (kSink != kNoSink && masked) {
+#pragma unroll
+          for (int step = 0; step < 2; ++step) {
+            const int c = 2 * step + half;
+            const uint32_t bits = ~bits_below(c_first - 32 * c) & bits_below(c_limit - 32 * c);
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (!(bits & (1u << x))) pr2[step][x] = 0xff800000u;  // -inf: P = 0
+          }
+        }
 #pragma unroll
         for (int step = 0; step < 2; ++step) {
           const int c = 2 * step + half;
           uint32_t(&sr)[32] = pr2[step];
-          if (kSink != kNoSink && masked) {
-            const uint32_t bits = ~bits_below(c_first - 32 * c) & bits_below(c_limit - 32 * c);
-#pragma unroll
-            for (int x = 0; x < 32; ++x)
-              if (!(bits & (1u << x))) sr[x] = 0xff800000u;  // -inf: P = 0
-          } else if (masked) {
+          if (kSink == kNoSink && masked) {
 #pragma unroll
             for (int x = 0; x < 32; ++x)
               if (c * 32 + x < c_first || c * 32 + x >= c_limit) sr[x] = 0xff800000u;  // -inf: P = 0
@@ -998,31 +1003,28 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         }
         const bool masked = __any_sync(0xffffffffu, c_limit < kT || c_first > 0) || (vb[0] & vb[1]) != 0xffffffffu;
         const uint32_t tDS = tmem + lane_addr + C::kTmemDS + (it & 1) * 64;
+        if (kSink && masked) {
+#pragma unroll
+          for (int step = 0; step < 2; ++step) {
+            const int c = 2 * half + step;
+            const uint32_t bits = bits_below(c_limit - 32 * c) & (~bits_below(c_first - 32 * c) | bits_below(c_shown - 32 * c));
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (!(bits & (1u << x))) sr2[step][x] = 0xff800000u;  // -inf: P = 0
+          }
+        }
 #pragma unroll
         for (int step = 0; step < 2; ++step) {
           const int c = 2 * half + step;
           uint32_t(&sr)[32] = sr2[step];
           uint32_t(&dp)[32] = dp2[step];
-          bool dead = false;  // kSink: no row of the warp sees a key of the chunk
-          if (kSink && masked) {
-            const uint32_t bits = bits_below(c_limit - 32 * c) & (~bits_below(c_first - 32 * c) | bits_below(c_shown - 32 * c));
-            dead = __all_sync(0xffffffffu, bits == 0u);
-            if (!dead) {
-#pragma unroll
-              for (int x = 0; x < 32; ++x)
-                if (!(bits & (1u << x))) sr[x] = 0xff800000u;  // -inf: P = 0
-            }
-          } else if (masked) {
+          if (!kSink && masked) {
 #pragma unroll
             for (int x = 0; x < 32; ++x)
               if (c * 32 + x >= c_limit || c * 32 + x < c_first || !((vb[x & 1] >> ((32 * step + x) >> 1)) & 1u))
                 sr[x] = 0xff800000u;  // -inf: P = 0
           }
           uint32_t pk_s[16];
-          if (dead) {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) pk_s[x] = 0u;
-          } else
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
             const uint64_t t2 = fma_f32x2(pack_u32x2(sr[2 * x], sr[2 * x + 1]), sl2x2, nl2);

@@ -800,22 +800,18 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         int limit = p.kv_seq - key0;
         if (p.causal) limit = min(limit, row + 1 - key0);
         const int first = (kMask != kNoMask && p.window > 0) ? row - p.window + 1 - key0 : 0;
-        uint32_t dead = 0;  // kSinkMask: bit c: no row of the warp sees a key of the tile's c-th 32
         if (kMask == kSinkMask) {
-          // ... and [0, shown), the first tokens.  A quarter of the tile at a time, as bits: most quarters of a tile at the
-          // window's ends, and all but the first of a tile of first tokens, are seen by all of the warp's rows or by none.
+          // ... and [0, shown), the first tokens; 32 keys at a time as bits.  (Leaving out the exponentials of 32 keys that no
+          // row of the warp sees, three quarters of a tile of four first tokens, costs more in branches, which keep the
+          // chunks' instructions apart, than it saves: 9001 rows, 32/8 heads of 128, window 1024 186 us against 172.)
           if (__any_sync(0xffffffffu, limit < kBN || first > 0)) {
             const int shown = p.n_sink - key0;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const uint32_t bits = bits_below(limit - 32 * c) & (~bits_below(first - 32 * c) | bits_below(shown - 32 * c));
-              if (__all_sync(0xffffffffu, bits == 0u)) {
-                dead |= 1u << c;
-              } else if (__any_sync(0xffffffffu, bits != 0xffffffffu)) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (!(bits & (1u << i))) sr[c][i] = 0xff800000u;  // -inf
-              }
+              for (int i = 0; i < 32; ++i)
+                if (!(bits & (1u << i))) sr[c][i] = 0xff800000u;  // -inf
             }
           }
         } else if (limit < kBN || first > 0) {
@@ -839,10 +835,6 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           mxa[c] = max3_f32(__uint_as_float(sr[c][0]), __uint_as_float(sr[c][1]), __uint_as_float(sr[c][2]));
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          if (kMask == kSinkMask && ((dead >> c) & 1u)) {
-            mxa[c] = -INFINITY;
-            continue;
-          }
 #pragma unroll
           for (int i = 3; i + 1 < 32; i += 2)
             mxa[c] = max3_f32(mxa[c], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
@@ -882,12 +874,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 #pragma unroll
         for (int c = 0; c < kBN / 32; ++c) {
           uint32_t pk[16];
-          if (kMask == kSinkMask && ((dead >> c) & 1u)) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pk[i] = 0u;
-          } else {
-            exp_chunk<kMask != kNoMask ? 0 : kExpPolyPairs>(sr[c], sl2x2, negx2, pk, sum_a, sum_b);
-          }
+          exp_chunk<kMask != kNoMask ? 0 : kExpPolyPairs>(sr[c], sl2x2, negx2, pk, sum_a, sum_b);
           tmem_st16(tS + c * 16, pk);
           if (c == 1) {  // keys 0..63 of P are in tensor memory: the first half of PV may start
             tmem_wait_st();
