@@ -21,7 +21,6 @@
 namespace tyr {
 namespace {
 
-constexpr int kSelectThreads = 1024;
 constexpr int kMoveThreads = 256;
 
 struct EvictParams {
@@ -46,24 +45,25 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// Positions a CTA holds at once, kItems of them per thread, position x * kSelectThreads + thread as item x.
-constexpr int kItems = 16, kSegment = kItems * kSelectThreads, kAhead = 4;
+// Positions a thread holds at once: position k * kThreads + thread as item k.  kAhead of them are fetched before the length is known.
+constexpr int kItems = 16, kAhead = 4;
 
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) evict_select_kernel(const EvictParams p) {
+  constexpr int kSegment = kItems * kThreads;
   __shared__ uint32_t hist[256];
-  __shared__ uint32_t counts[kItems * kSelectThreads / 32];  // per item and warp, in the order of the positions: over, equal << 16
-  __shared__ uint32_t warp_sums[kSelectThreads / 32];
+  __shared__ uint32_t counts[kItems * kThreads / 32];  // per item and warp, in the order of the positions: over, equal << 16
+  __shared__ uint32_t warp_sums[kThreads / 32];
   __shared__ uint32_t sel_digit, sel_left;
   grid_launch_dependents();
   grid_dependency_wait();
   const int hkv = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   float* w = p.weights + b * p.w_stride_b + hkv * p.w_stride_h;
-  // a segment's weights stay in registers over all passes where there is only one; its first positions are fetched
-  // before the length is known (the array has max_len of them)
+  // a segment's weights stay in registers over all passes where there is only one (the array has max_len entries)
   float x[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    const int i = k * kSelectThreads + tid;
+    const int i = k * kThreads + tid;
     x[k] = k < kAhead && i < p.max_len ? w[i] : 0.f;
   }
   const int raw = p.kv_lens[b], n = min(max(raw, 0), p.max_len);
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     p.new_lens[b] = min(n, p.n_keep);
   }
   if (n <= p.n_keep) {  // within the budget
-    for (int i = tid; i < p.n_keep; i += kSelectThreads) kept[i] = i < n ? i : -1;
+    for (int i = tid; i < p.n_keep; i += kThreads) kept[i] = i < n ? i : -1;
     return;
   }
   const int lo = p.n_sink, hi = n - p.n_recent;        // the candidates' positions
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
       if (k < k0) continue;
-      const int i = i0 + k * kSelectThreads + tid;
+      const int i = i0 + k * kThreads + tid;
       x[k] = i < n ? w[i] : 0.f;
     }
   };
@@ -101,8 +101,8 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
         if (!one_segment) load(i0, 0);
 #pragma unroll
         for (int k = 0; k < kItems; ++k) {
-          const int i = i0 + k * kSelectThreads + tid;
-          if (i0 + k * kSelectThreads >= hi) break;
+          const int i = i0 + k * kThreads + tid;
+          if (i0 + k * kThreads >= hi) break;
           const uint32_t u = ordered(x[k]);
           if (i >= lo && i < hi && (u & above) == T) atomicAdd(&hist[(u >> shift) & 255u], 1u);
         }
@@ -144,9 +144,9 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     uint32_t over_bits = 0, equal_bits = 0;  // of this thread's items
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
-      const int i = i0 + k * kSelectThreads + tid;
-      if (i0 + k * kSelectThreads >= n) {
-        if (lane == 0) counts[k * (kSelectThreads / 32) + warp] = 0u;
+      const int i = i0 + k * kThreads + tid;
+      if (i0 + k * kThreads >= n) {
+        if (lane == 0) counts[k * (kThreads / 32) + warp] = 0u;
         continue;
       }
       const uint32_t u = ordered(x[k]);
@@ -155,12 +155,12 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
       over_bits |= (uint32_t)over << k;
       equal_bits |= (uint32_t)equal << k;
       const uint32_t c = __popc(__ballot_sync(0xffffffffu, over)) | __popc(__ballot_sync(0xffffffffu, equal)) << 16;
-      if (lane == 0) counts[k * (kSelectThreads / 32) + warp] = c;
+      if (lane == 0) counts[k * (kThreads / 32) + warp] = c;
     }
     __syncthreads();  // every weight of the segment is in a register, every count in shared memory
     // exclusive prefix sums of the counts (at most kSegment of either kind: 16 bits each)
-    constexpr int kCounts = kItems * kSelectThreads / 32;
-    static_assert(kCounts <= kSelectThreads && kSegment < 65536, "one count per thread");
+    constexpr int kCounts = kItems * kThreads / 32;
+    static_assert(kCounts <= kThreads && kSegment < 65536, "one count per thread");
     const uint32_t mine = tid < kCounts ? counts[tid] : 0u;
     uint32_t sum = mine;
 #pragma unroll
@@ -180,14 +180,14 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
-      if (i0 + k * kSelectThreads >= n) break;
+      if (i0 + k * kThreads >= n) break;
       const bool over = (over_bits >> k) & 1u, equal = (equal_bits >> k) & 1u;
-      const uint32_t lower = (1u << lane) - 1u, c = counts[k * (kSelectThreads / 32) + warp];
+      const uint32_t lower = (1u << lane) - 1u, c = counts[k * (kThreads / 32) + warp];
       const uint32_t over_at = over_before + (c & 0xffffu) + __popc(__ballot_sync(0xffffffffu, over) & lower);
       const uint32_t equal_at = equal_before + (c >> 16) + __popc(__ballot_sync(0xffffffffu, equal) & lower);
       if (over || (equal && equal_at < left)) {
         const uint32_t to = over_at + min(equal_at, left);
-        kept[to] = i0 + k * kSelectThreads + tid;
+        kept[to] = i0 + k * kThreads + tid;
         w[to] = x[k];  // (at most the key's own position)
       }
     }
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     equal_before += total >> 16;
     __syncthreads();  // (the counts are the next segment's)
   }
-  for (int i = p.n_keep + tid; i < n; i += kSelectThreads) w[i] = 0.f;
+  for (int i = p.n_keep + tid; i < n; i += kThreads) w[i] = 0.f;
 }
 
 // kLanes threads of 16 bytes make one row of a CTA's columns; kRows rows of each thread are in flight, and the next step's
@@ -287,7 +287,11 @@ int launch_paged_evict(const TyrAttnEvictArgs& a, int* status, cudaStream_t st) 
   p.n_sink = a.n_sink;
   for (int i = 0; i < 3; ++i) { p.ks[i] = a.k_stride[i]; p.vs[i] = a.v_stride[i]; }
   p.status = status;
-  cudaError_t e = launch_overlapped(evict_select_kernel, dim3(a.n_kv_head, a.batch), dim3(kSelectThreads), 0, st, 1, p);
+  // Half as many threads, two CTAs per SM, while they hold a sequence: 64 sequences of 1000 keys, 8 KV heads, both launches
+  // 56.9 -> 47.1 us, one of 2049 11.1 -> 10.4; with half as many for 32 sequences of up to 16 K 155.8 -> 161.9.
+  const bool few = a.max_kv_seq <= kItems * 512;
+  cudaError_t e = launch_overlapped(few ? evict_select_kernel<512> : evict_select_kernel<1024>, dim3(a.n_kv_head, a.batch),
+                                    dim3(few ? 512 : 1024), 0, st, 1, p);
   count_launch();
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
