@@ -365,6 +365,18 @@ def test_evict_ties_and_odd_weights(kind):
         evict_case([5000, 4100], 2, 64, 16, n_keep, 100, 4, w, seed=1)
 
 
+# what one CTA holds, clusters of 2 to 16, and past them; ties across the CTAs' borders, sequences that end in an early CTA
+@pytest.mark.parametrize("lens,n_keep", [([16384, 8192, 8193], 5000), ([16385, 16384, 20], 16384), ([40000, 17000], 16000), ([140000, 100000, 3000], 70000),
+                                         ([262144, 200000], 1000), ([262145, 300], 200000)])
+@pytest.mark.parametrize("ties", [False, True])
+def test_evict_long(lens, n_keep, ties):
+    g = torch.Generator().manual_seed(n_keep)
+    w = torch.rand(len(lens), 1, max(lens), generator=g)
+    if ties:
+        w = (w * 3).floor()
+    evict_case(lens, 1, 64, 64, n_keep, n_keep // 3, 7, w, seed=4)
+
+
 def test_evict_large_and_reported():
     g = torch.Generator().manual_seed(11)
     evict_case([40000, 9000], 2, 64, 64, 8192, 1000, 4, torch.rand(2, 2, 40000, generator=g), seed=2)

@@ -1,9 +1,13 @@
 // Eviction from a paged KV cache by accumulated attention weight: per (sequence, KV head) the first n_sink and the last
 // n_recent keys stay, and of the others those with the greatest sums of weights, up to n_keep keys in all.
 //
+// Bound: HBM, one read and one write of every row that moves (32 sequences of 2 K to 16 K keys down to 4096, 8 KV heads of 128,
+// 926 MB: 154 us, 6.0 TB/s, of which the selection's 26 us run ahead); one short sequence is two launches' latency
+// (2049 keys down to 1024: 10.5 us).
+//
 // Two launches:
-//   evict_select_kernel : one CTA per (sequence, KV head) finds the weight T of the last key that stays by radix selection
-//                         (four passes over 8 bits of the weights' order-preserving integers), then one pass in the order
+//   evict_select_kernel : one CTA or cluster of CTAs per (sequence, KV head) finds the weight T of the last key that stays by radix selection
+//                         (passes over digits of the weights' order-preserving integers), then one pass in the order
 //                         of the positions writes the list of the kept ones and moves their weights.  Of the keys
 //                         that weigh exactly T the lower positions stay.
 //   evict_move_kernel   : moves the kept K and V rows to the front.  A kept key's new row is at most its old one, so a
@@ -13,6 +17,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "attn_internal.h"
 #include "fast_div.h"
@@ -35,6 +40,7 @@ struct EvictParams {
   int32_t *new_lens, *kept;
   int n_kv_head, max_len, n_keep, n_recent, n_sink;
   int64_t ks[3], vs[3];  // page, head, row
+  int ranks;             // CTAs of a cluster that share a (sequence, KV head)
   int* status;
 };
 
@@ -45,121 +51,154 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// Positions a thread holds at once: position k * kThreads + thread as item k.  kAhead of them are fetched before the length is known.
+// Positions a thread holds at once: position k * kThreads + thread as item k.
 constexpr int kItems = 16, kAhead = 4;
-
-template <int kThreads>
+constexpr int kMaxCluster = 16;
+// kCluster: the CTAs of a cluster share the (sequence, KV head), a segment of kItems * kThreads positions each, so that a
+// long sequence's weights stay in registers too; the histograms and counts are added through distributed shared memory.
+// Otherwise one CTA, which reads the weights again in every pass where they are more than a segment.
+// kBits: of a digit; the first digit of 11 has the sign, the exponent and two bits of the mantissa, of 8, which weights fill half a
+// dozen values of, it has most of the exponent.  Three passes of 11 bits are faster where there are many keys, four of 8, with an
+// eighth of the bins to clear and to add up, where there are few (the launch says which).
+template <int kThreads, bool kCluster, int kBits>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) evict_select_kernel(const EvictParams p) {
-  constexpr int kSegment = kItems * kThreads;
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t counts[kItems * kThreads / 32];  // per item and warp, in the order of the positions: over, equal << 16
-  __shared__ uint32_t warp_sums[kThreads / 32];
-  __shared__ uint32_t sel_digit, sel_left;
+  constexpr int kSegment = kItems * kThreads, kWarps = kThreads / 32, kBins = 1 << kBits, kPasses = (32 + kBits - 1) / kBits;
+  __shared__ __align__(16) uint32_t hist[2][kBins];             // of this CTA, alternating from pass to pass
+  __shared__ uint32_t counts[kItems * kWarps];  // per item and warp, in the order of the positions: over, equal << 16
+  __shared__ uint32_t warp_sums[kWarps], bin_sums[(kBins / 8 + 31) / 32];
+  __shared__ uint32_t sel_digit, sel_left, own_total;
   grid_launch_dependents();
   grid_dependency_wait();
-  const int hkv = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = kCluster ? (int)cluster_rank() : 0, ranks = kCluster ? p.ranks : 1;
+  const int hkv = kCluster ? blockIdx.x / ranks : blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   float* w = p.weights + b * p.w_stride_b + hkv * p.w_stride_h;
-  // a segment's weights stay in registers over all passes where there is only one (the array has max_len entries)
-  float x[kItems];
+  const int i_own = rank * kSegment;              // the first position of this CTA's (first) segment
+  uint32_t u[kItems];
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    const int i = k * kThreads + tid;
-    x[k] = k < kAhead && i < p.max_len ? w[i] : 0.f;
+  for (int k = 0; k < kAhead; ++k) {  // on their way while the length is fetched (the array has max_len entries)
+    const int i = i_own + k * kThreads + tid;
+    u[k] = i < p.max_len ? __float_as_uint(w[i]) : 0u;
   }
+  for (int q = tid; q < kBins / 4; q += kThreads) reinterpret_cast<uint4*>(hist[0])[q] = make_uint4(0u, 0u, 0u, 0u);
   const int raw = p.kv_lens[b], n = min(max(raw, 0), p.max_len);
   int32_t* kept = p.kept + ((int64_t)b * p.n_kv_head + hkv) * p.n_keep;
-  if (hkv == 0 && tid == 0) {
+  if (hkv == 0 && rank == 0 && tid == 0) {
     if (raw != n) atomicOr(p.status, kStatusOutOfRange);
     p.new_lens[b] = min(n, p.n_keep);
   }
-  if (n <= p.n_keep) {  // within the budget
-    for (int i = tid; i < p.n_keep; i += kThreads) kept[i] = i < n ? i : -1;
+  if (n <= p.n_keep) {  // within the budget (the whole cluster)
+    for (int i = rank * kThreads + tid; i < p.n_keep; i += ranks * kThreads) kept[i] = i < n ? i : -1;
     return;
   }
-  const int lo = p.n_sink, hi = n - p.n_recent;        // the candidates' positions
-  const uint32_t m = p.n_keep - p.n_sink - p.n_recent;  // how many of them stay: fewer than there are
+  // The weights as integers in their order; what always stays is above all of them, and what lies behind the last
+  // position is 0 like a NaN, whose equals before it are enough.  A segment's stay in registers over all passes.
+  const int lo = p.n_sink, hi = n - p.n_recent;
   auto load = [&](int i0, int k0) {
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
-      if (k < k0) continue;
       const int i = i0 + k * kThreads + tid;
-      x[k] = i < n ? w[i] : 0.f;
+      if (k >= k0) u[k] = i < n ? __float_as_uint(w[i]) : 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      if (i0 + k * kThreads >= n) break;
+      const int i = i0 + k * kThreads + tid;
+      u[k] = i >= n ? 0u : i < lo || i >= hi ? 0xffffffffu : ordered(__uint_as_float(u[k]));
     }
   };
-  const bool one_segment = n <= kSegment;
-  load(0, kAhead);
-  // T: the m-th greatest; `left`: how many of the keys equal to it stay
-  uint32_t T = 0xffffffffu, left = 0;
-  if (m > 0) {
-    T = 0;
-    left = m;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      const uint32_t above = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-      for (int i0 = 0; i0 < hi; i0 += kSegment) {
-        if (!one_segment) load(i0, 0);
+  const bool held = kCluster || n <= kSegment;    // every weight is in its thread's registers
+  const int i_end = kCluster ? min(n, i_own + kSegment) : n;
+  load(i_own, kAhead);
+  // T: the n_keep-th greatest; `left`: how many of those equal to it stay
+  uint32_t T = 0, left = p.n_keep;
+  __syncthreads();
+  for (int pass = 0; pass < kPasses; ++pass) {
+    const int shift = max(32 - kBits * (pass + 1), 0);  // (the last digit may be shorter)
+    const uint32_t above = pass == 0 ? 0u : 0xffffffffu << (32 - kBits * pass), digits = ~above >> shift;
+    uint32_t* own = hist[pass & 1];
+    for (int i0 = i_own; i0 < i_end; i0 += kSegment) {
+      if (!held) load(i0, 0);
 #pragma unroll
-        for (int k = 0; k < kItems; ++k) {
-          const int i = i0 + k * kThreads + tid;
-          if (i0 + k * kThreads >= hi) break;
-          const uint32_t u = ordered(x[k]);
-          if (i >= lo && i < hi && (u & above) == T) atomicAdd(&hist[(u >> shift) & 255u], 1u);
-        }
+      for (int k = 0; k < kItems; ++k) {
+        if (i0 + k * kThreads >= n) break;
+        if ((u[k] & above) == T) atomicAdd(&own[(u[k] >> shift) & digits], 1u);
       }
-      __syncthreads();
-      if (tid < 32) {
-        // lane l has digits 255 - 8 l .. 248 - 8 l: the greatest first
-        uint32_t c[8], sum = 0;
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          c[d] = hist[255 - 8 * tid - d];
-          sum += c[d];
-        }
-        uint32_t before = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t y = __shfl_up_sync(0xffffffffu, before, o);
-          if (tid >= o) before += y;
-        }
-        before -= sum;
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          if (before < left && before + c[d] >= left) {
-            sel_digit = 255 - 8 * tid - d;
-            sel_left = left - before;
-          }
-          before += c[d];
-        }
-      }
-      __syncthreads();
-      T |= sel_digit << shift;
-      left = sel_left;
     }
+    // Behind this barrier every CTA has read the other histogram (it belongs to the pass before): it is the next pass's.
+    if (kCluster) cluster_sync();
+    else __syncthreads();
+    // thread t has digits kBins - 1 - 8 t .. kBins - 8 - 8 t: the greatest first
+    uint32_t c[8], sum = 0, before = 0;
+    if (tid < kBins / 8) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t at = smem_u32(&own[kBins - 8 - 8 * tid + 4 * (1 - h)]);
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        for (int r = 0; r < ranks; ++r) {
+          const uint4 y = kCluster ? cluster_ld_u32x4(cluster_map(at, r)) : *reinterpret_cast<const uint4*>(&own[kBins - 8 - 8 * tid + 4 * (1 - h)]);
+          v.x += y.x;
+          v.y += y.y;
+          v.z += y.z;
+          v.w += y.w;
+        }
+        c[4 * h] = v.w;
+        c[4 * h + 1] = v.z;
+        c[4 * h + 2] = v.y;
+        c[4 * h + 3] = v.x;
+      }
+#pragma unroll
+      for (int d = 0; d < 8; ++d) sum += c[d];
+      before = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += y;
+      }
+      if (lane == 31) bin_sums[warp] = before;
+      before -= sum;
+    } else {
+      for (int q = tid - kBins / 8; q < kBins / 4; q += kThreads - kBins / 8)
+        reinterpret_cast<uint4*>(hist[(pass & 1) ^ 1])[q] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (kBins / 8 > 32) __syncthreads();
+    if (tid < kBins / 8) {
+      for (int v = 0; v < warp; ++v) before += bin_sums[v];
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        if (before < left && before + c[d] >= left) {
+          sel_digit = kBins - 1 - 8 * tid - d;
+          sel_left = left - before;
+        }
+        before += c[d];
+      }
+    }
+    __syncthreads();
+    T |= sel_digit << shift;
+    left = sel_left;
+    // (sel_* and bin_sums are written again only behind the next pass's first barrier)
   }
-  // in the order of the positions: a key stays if it always does, weighs more than T, or is one of the first `left` equal to T
+  // in the order of the positions: a key stays if it is above T, or one of the first `left` equal to T
   uint32_t over_before = 0, equal_before = 0;
-  for (int i0 = 0; i0 < n; i0 += kSegment) {
-    if (!one_segment) load(i0, 0);
+  for (int i0 = i_own; kCluster ? i0 == i_own : i0 < n; i0 += kSegment) {
+    if (!held) load(i0, 0);
     uint32_t over_bits = 0, equal_bits = 0;  // of this thread's items
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
-      const int i = i0 + k * kThreads + tid;
       if (i0 + k * kThreads >= n) {
-        if (lane == 0) counts[k * (kThreads / 32) + warp] = 0u;
+        if (lane == 0) counts[k * kWarps + warp] = 0u;
         continue;
       }
-      const uint32_t u = ordered(x[k]);
-      const bool candidate = i >= lo && i < hi;
-      const bool over = i < lo || (i >= hi && i < n) || (candidate && u > T), equal = candidate && u == T;
+      const int i = i0 + k * kThreads + tid;
+      const bool over = u[k] > T, equal = u[k] == T;
       over_bits |= (uint32_t)over << k;
       equal_bits |= (uint32_t)equal << k;
       const uint32_t c = __popc(__ballot_sync(0xffffffffu, over)) | __popc(__ballot_sync(0xffffffffu, equal)) << 16;
-      if (lane == 0) counts[k * (kThreads / 32) + warp] = c;
+      if (lane == 0) counts[k * kWarps + warp] = c;
+      if ((over || equal) && i < n) u[k] = __float_as_uint(w[i]);  // the weight itself, its bits as they are
     }
-    __syncthreads();  // every weight of the segment is in a register, every count in shared memory
+    __syncthreads();
     // exclusive prefix sums of the counts (at most kSegment of either kind: 16 bits each)
-    constexpr int kCounts = kItems * kThreads / 32;
+    constexpr int kCounts = kItems * kWarps;
     static_assert(kCounts <= kThreads && kSegment < 65536, "one count per thread");
     const uint32_t mine = tid < kCounts ? counts[tid] : 0u;
     uint32_t sum = mine;
@@ -177,25 +216,38 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) evict_select_kernel
       total += warp_sums[v];
     }
     if (tid < kCounts) counts[tid] = base + sum - mine;
-    __syncthreads();
+    // Behind this barrier every weight of the segment (of the sequence, in a cluster) that stays is in a register: what is
+    // written below may be another thread's position.
+    if (kCluster) {
+      if (tid == 0) own_total = total;
+      cluster_sync();
+      for (int r = 0; r < rank; ++r) {
+        const uint32_t t = cluster_ld_u32(cluster_map(smem_u32(&own_total), r));
+        over_before += t & 0xffffu;
+        equal_before += t >> 16;
+      }
+    } else {
+      __syncthreads();
+    }
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
       if (i0 + k * kThreads >= n) break;
       const bool over = (over_bits >> k) & 1u, equal = (equal_bits >> k) & 1u;
-      const uint32_t lower = (1u << lane) - 1u, c = counts[k * (kThreads / 32) + warp];
+      const uint32_t lower = (1u << lane) - 1u, c = counts[k * kWarps + warp];
       const uint32_t over_at = over_before + (c & 0xffffu) + __popc(__ballot_sync(0xffffffffu, over) & lower);
       const uint32_t equal_at = equal_before + (c >> 16) + __popc(__ballot_sync(0xffffffffu, equal) & lower);
       if (over || (equal && equal_at < left)) {
         const uint32_t to = over_at + min(equal_at, left);
         kept[to] = i0 + k * kThreads + tid;
-        w[to] = x[k];  // (at most the key's own position)
+        w[to] = __uint_as_float(u[k]);  // (at most the key's own position)
       }
     }
     over_before += total & 0xffffu;
     equal_before += total >> 16;
-    __syncthreads();  // (the counts are the next segment's)
+    if (!kCluster) __syncthreads();  // (the counts are the next segment's)
   }
-  for (int i = p.n_keep + tid; i < n; i += kThreads) w[i] = 0.f;
+  for (int i = max(i_own, p.n_keep) + tid; i < i_end; i += kThreads) w[i] = 0.f;
+  if (kCluster) cluster_sync();  // no CTA's shared memory goes away while another still reads it
 }
 
 // kLanes threads of 16 bytes make one row of a CTA's columns; kRows rows of each thread are in flight, and the next step's
@@ -263,6 +315,19 @@ cudaError_t launch_move(const EvictParams& p, int batch, int head_dim, cudaStrea
   return launch_overlapped(evict_move_kernel<kLanes>, dim3(2 * slices, p.n_kv_head, batch), dim3(kMoveThreads), 0, st, 1, p, slices);
 }
 
+cudaError_t allow_clusters_of_16() {
+  static std::atomic<bool> set[64] = {};  // per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!set[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(evict_select_kernel<1024, true, 11>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) set[dev].store(true, std::memory_order_release);
+  }
+  return e;
+}
+
 }  // namespace
 
 int launch_paged_evict(const TyrAttnEvictArgs& a, int* status, cudaStream_t st) {
@@ -288,10 +353,22 @@ int launch_paged_evict(const TyrAttnEvictArgs& a, int* status, cudaStream_t st) 
   for (int i = 0; i < 3; ++i) { p.ks[i] = a.k_stride[i]; p.vs[i] = a.v_stride[i]; }
   p.status = status;
   // Half as many threads, two CTAs per SM, while they hold a sequence: 64 sequences of 1000 keys, 8 KV heads, both launches
-  // 56.9 -> 47.1 us, one of 2049 11.1 -> 10.4; with half as many for 32 sequences of up to 16 K 155.8 -> 161.9.
+  // 56.9 -> 47.0 us, one of 2049 11.1 -> 10.5; with half as many for 32 sequences of up to 16 K 155.8 -> 161.9.  Digits of 11 bits
+  // there: one of 2049 11.2 us.  Past what one CTA holds a cluster, up to 16 times as much (one sequence of 30000 keys 50.0 ->
+  // 37.5 us, of 100000 the first launch alone 97 -> 28); what is longer still is one CTA's, in segments.
+  const int segment = kItems * 1024;
   const bool few = a.max_kv_seq <= kItems * 512;
-  cudaError_t e = launch_overlapped(few ? evict_select_kernel<512> : evict_select_kernel<1024>, dim3(a.n_kv_head, a.batch),
-                                    dim3(few ? 512 : 1024), 0, st, 1, p);
+  p.ranks = 1;
+  while (p.ranks < kMaxCluster && (long long)p.ranks * segment < a.max_kv_seq) p.ranks *= 2;
+  if ((long long)p.ranks * segment < a.max_kv_seq) p.ranks = 1;
+  cudaError_t e;
+  if (p.ranks > 1) {
+    if ((e = allow_clusters_of_16()) != cudaSuccess) return (int)e;
+    e = launch_overlapped(evict_select_kernel<1024, true, 11>, dim3(a.n_kv_head * p.ranks, a.batch), dim3(1024), 0, st, p.ranks, p);
+  } else {
+    e = launch_overlapped(few ? evict_select_kernel<512, false, 8> : evict_select_kernel<1024, false, 11>, dim3(a.n_kv_head, a.batch),
+                          dim3(few ? 512 : 1024), 0, st, 1, p);
+  }
   count_launch();
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
