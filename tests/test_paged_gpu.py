@@ -452,3 +452,94 @@ def test_generating_loop_with_a_budget(window):
                     assert ids == plain_evict(None, None, before[b, h:h + 1, :len(held[b][h][0])].cpu(), budget, 20, 4)[0]
                     held[b][h] = tuple(t[ids] for t in held[b][h])
     assert int(cached.max()) < int(text.max())                # the budget was passed on the way
+
+
+def test_table_and_lengths_rewritten_between_calls():
+    """The table and the lengths are the device's: each call sees what the kernel before it on the stream wrote."""
+    page, n_pages, hkv, d = 16, 400, 2, 64
+    g = torch.Generator().manual_seed(5)
+    kp, vp = (torch.randn(n_pages, hkv, page, d, generator=g).bfloat16() for _ in range(2))
+    kd, vd = kp.to(DEV), vp.to(DEV)
+    q = randn(3, 4, d, seed=6)
+    plans = [(torch.stack([torch.randperm(n_pages, generator=g)[:60] for _ in range(3)]).int(), torch.randint(1, 961, (3,), generator=g).int())
+             for _ in range(12)]
+    on_dev = [(t.to(DEV), n.to(DEV)) for t, n in plans]
+    table, lens = torch.zeros(3, 60, dtype=torch.int32, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
+    ws = torch.empty(tnn.paged_decode_workspace_bytes(q, kd, vd, table, lens), dtype=torch.uint8, device=DEV)
+    out = []
+    for t, n in on_dev:
+        table.copy_(t)
+        lens.copy_(n)
+        out.append(tnn.flashDecodePaged(q, kd, vd, table, lens, workspace=ws))
+    for (t, n), (o, lse) in zip(plans, out):
+        for b in range(3):
+            j = torch.arange(int(n[b]))
+            at = t[b, j // page].long()
+            check_token(o[b], lse[b], definition(q[b], kp[at, :, j % page], vp[at, :, j % page]))
+
+
+def test_calls_on_two_streams_with_workspaces_of_their_own():
+    lens = [30000, 20000]
+    c = Cache(lens, 2, 128, 16, seed=12)
+    qs = [randn(2, 8, 128, seed=s) for s in (1, 2)]
+    want = [tnn.flashDecodePaged(q, c.kp, c.vp, c.table_dev, c.lens_dev, max_kv_seq=30000) for q in qs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in qs], [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(tnn.flashDecodePaged(qs[i], c.kp, c.vp, c.table_dev, c.lens_dev, max_kv_seq=30000))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i][0]) and torch.equal(l, want[i][1]) for o, l in got[i])
+
+
+def test_loop_with_eviction_as_a_graph():
+    """One captured step (append, attention with sums, the counters) replayed, and a captured eviction, against the eager calls."""
+    hq, hkv, d, page, cap = 8, 2, 64, 16, 320
+    xs = [(randn(2, 1, hkv, d, seed=10 + i), randn(2, 1, hkv, d, seed=60 + i), randn(2, hq, d, seed=110 + i)) for i in range(30)]
+    table = torch.randperm(40, generator=torch.Generator().manual_seed(1)).int().view(2, 20).to(DEV)
+
+    def run(graphs):
+        kp, vp = (torch.zeros(40, hkv, page, d, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        sums = torch.zeros(2, hkv, cap, device=DEV)
+        n, n2 = torch.tensor([3, 200], dtype=torch.int32, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
+        kept = torch.zeros(2, hkv, 150, dtype=torch.int32, device=DEV)
+        xk, xv, q = (torch.zeros_like(t) for t in xs[0])
+        o, lse = torch.zeros(2, hq, d, dtype=torch.bfloat16, device=DEV), torch.zeros(2, hq, device=DEV)
+        ws = torch.empty(tnn.paged_decode_workspace_bytes(q, kp, vp, table, n, cap, weights=sums), dtype=torch.uint8, device=DEV)
+
+        def step():
+            tnn.qkPrologue(xk, kp, positions=n, page_table=table)
+            tnn.qkPrologue(xv, vp, positions=n, page_table=table)
+            n.add_(1)
+            tnn.flashDecodePaged(q, kp, vp, table, n, max_kv_seq=cap, weights=sums, out=o, lse=lse, workspace=ws)
+
+        def evict():
+            tnn.evictPaged(kp, vp, table, n, sums, 150, 40, 4, max_kv_seq=cap, new_lens=n2, kept=kept)
+            n.copy_(n2)
+
+        if graphs:
+            calls = []
+            for f in (step, evict):
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    f()
+                calls.append(g.replay)
+            one, drop = calls
+        else:
+            one, drop = step, evict
+        seen = []
+        for i, x in enumerate(xs):
+            for to, t in zip((xk, xv, q), x):
+                to.copy_(t)
+            one()
+            seen += [o.clone(), lse.clone()]
+            if i % 10 == 9:
+                drop()
+                seen += [n.clone(), kept.clone(), kp.clone(), vp.clone(), sums.clone()]
+        return seen
+
+    eager, replayed = run(False), run(True)
+    assert len(eager) == len(replayed) and all(torch.equal(a, b) for a, b in zip(eager, replayed))
+    assert eager[-5].tolist() == [33, 150]
