@@ -2,8 +2,8 @@
 // n_recent keys stay, and of the others those with the greatest sums of weights, up to n_keep keys in all.
 //
 // Bound: HBM, one read and one write of every row that moves (32 sequences of 2 K to 16 K keys down to 4096, 8 KV heads of 128,
-// 926 MB: 154 us, 6.0 TB/s, of which the selection's 26 us run ahead); one short sequence is two launches' latency
-// (2049 keys down to 1024: 10.5 us).
+// 926 MB: 154 us, 6.0 TB/s; alone the selection is 24 us of that, the move 135, 6.9 TB/s); one short sequence is two
+// launches' latency (2049 keys down to 1024: 10.5 us, alone 6 and 3.4).
 //
 // Two launches:
 //   evict_select_kernel : one CTA or cluster of CTAs per (sequence, KV head) finds the weight T of the last key that stays by radix selection

@@ -41,7 +41,8 @@ struct PrologueParams {
   int* status;
 };
 
-// The same into a paged cache: os = {page, head, row}.
+// The same into a paged cache: os = {page, head, row}.  One table entry more per token: K and V of four prompts of 4096
+// tokens, 8 heads of 128 (136 MB) 28 us, 4.8 TB/s; K alone from and to L2 12.9 us, dense 12.7.
 struct PagedPrologueParams : PrologueParams {
   const int32_t* table;
   int64_t table_stride;
