@@ -594,20 +594,19 @@ PyObject* evict_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// x, out, norm_weight, cos, sin, positions, position0, eps, pe, out_at_row0, page_table, rows -> None
+// x, out, norm_weight, cos, sin, positions, position0, eps, pe, out_at_row0 [, page_table, rows] -> None
 PyObject* qk_prologue(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    require_count(n, 12);
+    if (n != 10) require_count(n, 12);
     const Tensor &x = tensor(args[0], "x"), &out = tensor(args[1], "out");
     require_cuda(x);
     require_cuda(out);
     if (x.dim() != 4 || out.dim() != 4 || x.scalar_type() != at::kBFloat16 || out.scalar_type() != at::kBFloat16)
       throw ValueError("x must be bf16 [B,S,H,D] and out bf16 [B,H,cap,D]");
-    const Tensor *table = maybe(args[10], "page_table"), *rows = maybe(args[11], "rows");
+    const Tensor *table = n == 10 ? nullptr : maybe(args[10], "page_table"), *rows = n == 10 ? nullptr : maybe(args[11], "rows");
     const int64_t B = x.size(0), S = x.size(1), H = x.size(2), D = x.size(3);
     if ((!table && out.size(0) != B) || out.size(1) != H || out.size(3) != D) throw ValueError("out does not match x");
-    TyrAttnPageTable pages;
-    std::memset(&pages, 0, sizeof(pages));
+    TyrAttnPageTable pages{};
     if (rows && !table) throw ValueError("rows goes with page_table");
     if (table) {
       fill_pages(pages, *table, out, B);

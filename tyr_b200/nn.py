@@ -391,7 +391,10 @@ def qkPrologue(x: torch.Tensor, out: torch.Tensor, norm_weight: Optional[torch.T
     keys were evicted from (`evictPaged`) is shorter than the text.  A row outside the table, or whose entry
     is no page of the pool, is skipped and sets the same status bit.
     """
-    _lib.calls().qk_prologue(x, out, norm_weight, cos, sin, positions, position0, eps, pe, out_at_row0, page_table, rows)
+    if page_table is None and rows is None:
+        _lib.calls().qk_prologue(x, out, norm_weight, cos, sin, positions, position0, eps, pe, out_at_row0)
+    else:
+        _lib.calls().qk_prologue(x, out, norm_weight, cos, sin, positions, position0, eps, pe, out_at_row0, page_table, rows)
     return out
 
 
