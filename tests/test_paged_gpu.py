@@ -543,3 +543,64 @@ def test_loop_with_eviction_as_a_graph():
     eager, replayed = run(False), run(True)
     assert len(eager) == len(replayed) and all(torch.equal(a, b) for a, b in zip(eager, replayed))
     assert eager[-5].tolist() == [33, 150]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rotary", ["none", "halves", "pairs"])
+def test_append_gives_the_bits_of_the_dense_call(d, rotary):
+    B, S, H, page = 2, 53, 6, 24
+    x, w = randn(B, S, H, d, seed=3).transpose(1, 2).contiguous().transpose(1, 2), torch.rand(d, device=DEV) + 0.5      # heads outer
+    start = torch.tensor([40, 5], dtype=torch.int32, device=DEV)
+    ang = torch.arange(100.0, device=DEV)[:, None] * torch.rand(d // 2, device=DEV)[None]
+    cos, sin = ang.cos().contiguous(), ang.sin().contiguous()
+    rot = {"none": {}, "halves": dict(cos=cos, sin=sin),
+           "pairs": dict(pe=torch.stack([cos, -sin, sin, cos], -1).view(1, 100, d // 2, 2, 2).contiguous())}[rotary]
+    dense = torch.zeros(B, H, 100, d, dtype=torch.bfloat16, device=DEV)
+    tnn.qkPrologue(x, dense, w, positions=start, **rot)
+    pool = torch.zeros(11, page, H, d, dtype=torch.bfloat16, device=DEV).transpose(1, 2)
+    table = torch.tensor([[9, 2, 7, 0, 4], [1, 10, 3, 8, 6]], dtype=torch.int32, device=DEV)
+    tnn.qkPrologue(x, pool, w, positions=start, page_table=table, **rot)
+    j = torch.arange(100, device=DEV)
+    for b in range(B):
+        assert torch.equal(pool[table[b, j // page].long(), :, j % page].transpose(0, 1), dense[b])
+
+
+def test_pages_far_apart():
+    """Pages 2^26 rows' worth of elements apart (offsets past 32 bits), V laid out in another way than K."""
+    hkv, d, page, n_pages = 2, 64, 16, 40
+    far = torch.empty(n_pages * 2 ** 26, dtype=torch.bfloat16, device=DEV)            # 5.4 GB
+    kp = far.as_strided((n_pages, hkv, page, d), (2 ** 26, 2 ** 20, 1024, 1))
+    vp = torch.zeros(hkv, n_pages, page, d, dtype=torch.bfloat16, device=DEV).transpose(0, 1)
+    table = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=DEV).view(1, n_pages)
+    xk, xv, q = randn(1, 600, hkv, d, seed=1), randn(1, 600, hkv, d, seed=2), randn(1, 4, d, seed=3)
+    tnn.qkPrologue(xk, kp, page_table=table)
+    tnn.qkPrologue(xv, vp, page_table=table)
+    lens, w = torch.tensor([600], dtype=torch.int32, device=DEV), torch.zeros(1, hkv, 640, device=DEV)
+    o, lse = tnn.flashDecodePaged(q, kp, vp, table, lens, weights=w)
+    want = definition(q[0], xk[0].cpu(), xv[0].cpu())
+    check_token(o[0], lse[0], want)
+    sums = w.clone()
+    lens, kept = tnn.evictPaged(kp, vp, table, lens, w, 300, 50, 4)
+    for h, left in enumerate(plain_evict(None, None, sums[0, :, :600].cpu(), 300, 50, 4)):
+        assert kept[0, h].tolist() == left
+        j = torch.arange(300, device=DEV)
+        at = table[0, j // page].long()
+        assert torch.equal(kp[at, h, j % page], xk[0, left, h]) and torch.equal(vp[at, h, j % page], xv[0, left, h])
+    del far
+
+
+def test_calls_on_the_other_device():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs in one process")
+    torch.cuda.set_device(0)
+    c = Cache([500, 20000], 2, 64, 16, seed=4)
+    q, w = randn(2, 4, 64, seed=5), torch.rand(2, 2, 20000, device=DEV)
+    got = []
+    for dev in ("cuda:0", "cuda:1"):
+        kp, vp, table, lens, ws, qd = (t.to(dev).clone() for t in (c.kp, c.vp, c.table_dev, c.lens_dev, w, q))
+        o, lse = tnn.flashDecodePaged(qd, kp, vp, table, lens, max_kv_seq=20000, weights=ws)
+        new, kept = tnn.evictPaged(kp, vp, table, lens, ws, 400, 30, 4, max_kv_seq=20000)
+        tnn.qkPrologue(qd.view(2, 1, 4, 64)[:, :, :2], kp, positions=new, page_table=table)
+        got.append([t.cpu() for t in (o, lse, ws, new, kept)] + [kp.cpu().view(torch.int16)])
+    assert torch.cuda.current_device() == 0 and tnn.device_status(1, True) == 0
+    assert all(torch.equal(a, b) for a, b in zip(*got))

@@ -158,3 +158,17 @@ def test_refusals():
         tnn.scaledDotProductAttentionGQAWindowSinks(q, k, v, window_size=0, n_sink=4)
     with pytest.raises(tnn.AttnError):
         tnn.attentionFwd(q[:, :, :32], k, v, window_size=4, n_sink=2)
+
+
+def test_on_the_other_device():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs in one process")
+    torch.cuda.set_device(0)
+    t = [randn(1, h, 2500, 64, seed=h + i) for i, h in enumerate((4, 2, 2, 4))]
+    got = []
+    for dev in ("cuda:0", "cuda:1"):
+        q, k, v, d_o = (x.to(dev) for x in t)
+        o, lse = tnn.attentionFwd(q, k, v, window_size=90, n_sink=4)
+        got.append([x.cpu() for x in (o, lse, *tnn.attentionBwd(q, k, v, o, lse, d_o, window_size=90, n_sink=4))])
+    assert torch.cuda.current_device() == 0 and tnn.device_status(1, True) == 0
+    assert all(torch.equal(a, b) for a, b in zip(*got))
