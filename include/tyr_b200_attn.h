@@ -49,8 +49,8 @@ extern "C" {
 /* bits of the per-device status word (tyr_b200_attn_device_status) */
 #define TYR_ATTN_STATUS_WAIT_TIMEOUT 1 /* a bounded in-kernel barrier wait ran out */
 #define TYR_ATTN_STATUS_ABORTED 2      /* a CTA left early because one of its roles gave up */
-#define TYR_ATTN_STATUS_OUT_OF_RANGE 4 /* a device-side position or length was outside its limits;
-                                          the offending rows were skipped (prologue) or clamped (decode) */
+#define TYR_ATTN_STATUS_OUT_OF_RANGE 4 /* a device-side position, length or page table entry was outside its limits; the
+                                          offending rows were skipped (prologue, eviction), clamped or made NaN (decode) */
 
 /* ------------------------------------------------------------------------
  * Prefill: O = softmax(Q K^T * scale + causal) V, per-row LSE.
@@ -243,6 +243,8 @@ int tyr_b200_attn_decode_static(const TyrAttnDecodeArgs* args, void* stream);
  * Only entries that hold a row the call touches are read: those behind a sequence's last row, and those of pages that
  * lie wholly between the first tokens and the window, may be anything (pages out of sight can be given back).
  * An entry outside [0, n_pages) that would be used sets TYR_ATTN_STATUS_OUT_OF_RANGE and is not followed.
+ * A page that several entries name (a shared prefix) can be read; rows that one call writes (append, eviction) must lie in
+ * pages that only one entry names, or which of the values they end up with is not said.
  * ---------------------------------------------------------------------- */
 typedef struct TyrAttnPageTable {
   const int32_t* table; /* DEVICE int32 [batch, max_pages] */
