@@ -377,6 +377,43 @@ def test_evict_long(lens, n_keep, ties):
     evict_case(lens, 1, 64, 64, n_keep, n_keep // 3, 7, w, seed=4)
 
 
+# enough (sequence, KV head) pairs for whole columns of 128 bytes per CTA; several steps of moves, ends inside a step
+@pytest.mark.parametrize("d,page,layout", [(64, 16, "phrd"), (128, 7, "prhd"), (256, 100, "hprd")])
+@pytest.mark.parametrize("n_keep,n_recent,n_sink", [(1, 0, 0), (130, 30, 4), (500, 0, 1), (127, 127, 0)])
+def test_evict_many(d, page, layout, n_keep, n_recent, n_sink):
+    g = torch.Generator().manual_seed(n_keep + d)
+    lens = [int(n) for n in torch.randint(0, 900, (40,), generator=g)]
+    w = torch.rand(40, 4, 900, generator=g)
+    evict_case(lens, 4, d, page, n_keep, n_recent, n_sink, w[:, :, :max(lens)].contiguous(), layout, seed=d)
+    assert 2 * (d // 64) * 4 * 40 >= 2 * torch.cuda.get_device_properties(0).multi_processor_count
+
+
+def test_evict_many_with_a_bad_page():
+    lens = [300] * 40
+    c = Cache(lens, 4, 64, 16, seed=3)
+    table = c.table_dev.clone()
+    table[7, 3] = c.kp.shape[0]                             # rows 48.. of sequence 7 have no place
+    k0 = c.kp.clone()
+    w = torch.rand(40, 4, 300, device=DEV)
+    sums = w.cpu()
+    _, kept = tnn.evictPaged(c.kp, c.vp, table, c.lens_dev, w, 100, 10)
+    assert tnn.device_status(0, True) == OUT_OF_RANGE
+    for b in range(40):
+        left = plain_evict(None, None, sums[b], 100, 10, 0)
+        for h in range(4):
+            assert kept[b, h].tolist() == left[h]
+            for i, src in enumerate(left[h]):
+                if b == 7 and (i // 16 == 3 or src // 16 == 3) and src != i:
+                    if i // 16 != 3:                        # stays as it was
+                        at, off = int(c.table[b, i // 16]), i % 16
+                        assert torch.equal(c.kp[at, h, off].view(torch.int16), k0[at, h, off].view(torch.int16))
+                    continue
+                if b in (0, 7, 39):
+                    assert torch.equal(c.kp[int(c.table[b, i // 16]), h, i % 16], c.k[b][src, h].to(DEV))
+    other = int(c.table[7, 3])                              # the page that the table no longer names
+    assert torch.equal(c.kp[other].view(torch.int16), k0[other].view(torch.int16))
+
+
 def test_evict_large_and_reported():
     g = torch.Generator().manual_seed(11)
     evict_case([40000, 9000], 2, 64, 64, 8192, 1000, 4, torch.rand(2, 2, 40000, generator=g), seed=2)

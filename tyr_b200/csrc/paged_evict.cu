@@ -2,7 +2,7 @@
 // n_recent keys stay, and of the others those with the greatest sums of weights, up to n_keep keys in all.
 //
 // Bound: HBM, one read and one write of every row that moves (32 sequences of 2 K to 16 K keys down to 4096, 8 KV heads of 128,
-// 926 MB: 154 us, 6.0 TB/s; alone the selection is 24 us of that, the move 135, 6.9 TB/s); one short sequence is two
+// 926 MB: 152 us, 6.1 TB/s; alone the selection is 24 us of that, the move 132, 7.0 TB/s); one short sequence is two
 // launches' latency (2049 keys down to 1024: 10.5 us, alone 6 and 3.4).
 //
 // Two launches:
@@ -11,9 +11,9 @@
 //                         of the positions writes the list of the kept ones and moves their weights.  Of the keys
 //                         that weigh exactly T the lower positions stay.
 //   evict_move_kernel   : moves the kept K and V rows to the front.  A kept key's new row is at most its old one, so a
-//                         CTA that walks the list forward may move in place: every row of a step is in registers
-//                         before the step's first store, and what a step writes lies below what later steps read.  Different
-//                         columns of a row do not meet, so the columns are spread over CTAs.
+//                         CTA that walks the list forward may move in place: every row of a step has been read before the
+//                         step's first store, and what a step writes lies below what later steps read.  Different
+//                         columns of a row do not meet, so the columns are spread over CTAs.  (evict_move_few_kernel: a launch of few.)
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -21,6 +21,7 @@
 
 #include "attn_internal.h"
 #include "fast_div.h"
+#include "mma_sync.cuh"
 #include "ptx_sm100.cuh"
 
 namespace tyr {
@@ -250,14 +251,87 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) evict_select_kernel
   if (kCluster) cluster_sync();  // no CTA's shared memory goes away while another still reads it
 }
 
-// kLanes threads of 16 bytes make one row of a CTA's columns; kRows rows of each thread are in flight, and the next step's
-// addresses (list entry, then table entry) are on their way while a step's rows arrive.
-template <int kLanes>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p, int slices) {
-  constexpr int kRows = 8, kGroup = kMoveThreads / kLanes, kStep = kRows * kGroup;  // kStep: rows a step moves
+// The columns of a row that one CTA moves, in lanes of 16 bytes.
+constexpr int kLanes = 8, kFewLanes = 2;
+
+// A step's rows come to shared memory asynchronously, two steps ahead of their stores.
+struct MoveCfg {
+  static constexpr int kRows = 4, kStages = 3;                    // rows of a thread in a step; steps in shared memory
+  static constexpr int kGroup = kMoveThreads / kLanes, kStep = kRows * kGroup;  // kStep: rows a step moves
+  static constexpr int kBufBytes = kStages * kRows * kMoveThreads * 16;
+  static constexpr int kSmemBytes = kBufBytes + kStages * kStep * 8;
+};
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
+  using C = MoveCfg;
+  constexpr int kRows = C::kRows, kStages = C::kStages, kGroup = C::kGroup, kStep = C::kStep;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint4* buf = reinterpret_cast<uint4*>(smem);                               // [stage][row of the thread][thread]
+  long long* to = reinterpret_cast<long long*>(smem + C::kBufBytes);         // [stage][row of the step]: where it goes, -1: nowhere
   grid_launch_dependents();
   grid_dependency_wait();
-  const int hkv = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int hkv = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, group = tid / kLanes, slices = gridDim.x / 2;
+  const int n = min(max(p.kv_lens[b], 0), p.max_len);
+  if (n <= p.n_keep) return;
+  const bool is_v = (int)blockIdx.x >= slices;
+  const int col = ((is_v ? blockIdx.x - slices : blockIdx.x) * kLanes + tid % kLanes) * 8;
+  const int64_t st0 = is_v ? p.vs[0] : p.ks[0], st2 = is_v ? p.vs[2] : p.ks[2];
+  __nv_bfloat16* base = (is_v ? p.v + hkv * p.vs[1] : p.k + hkv * p.ks[1]) + col;
+  const int32_t* kept = p.kept + ((int64_t)b * p.n_kv_head + hkv) * p.n_keep;
+  const int32_t* table = p.table + b * p.table_stride;
+  const int n_steps = (p.n_keep + kStep - 1) / kStep;
+  bool bad = false;
+  auto fetch = [&](int step) {
+    if (step < n_steps) {
+      int src[kRows], page_from[kRows], page_to[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const int i = step * kStep + r * kGroup + group;
+        src[r] = i < p.n_keep ? kept[i] : i;
+      }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const int i = step * kStep + r * kGroup + group;
+        page_from[r] = src[r] == i ? 0 : table[p.by_page.div(src[r])];  // (a row that stays where it is needs none)
+        page_to[r] = src[r] == i ? 0 : table[p.by_page.div(i)];
+      }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const int i = step * kStep + r * kGroup + group;
+        const bool out = (unsigned)page_from[r] >= (unsigned)p.n_pages || (unsigned)page_to[r] >= (unsigned)p.n_pages;  // not followed
+        const bool moves = src[r] != i && !out;
+        bad = bad || (src[r] != i && out);
+        if (moves)
+          cp_async16(smem_u32(&buf[(step % kStages * kRows + r) * kMoveThreads + tid]),
+                     base + page_from[r] * st0 + (src[r] - p.by_page.div(src[r]) * (int)p.by_page.d) * st2);
+        if (tid % kLanes == 0)
+          to[step % kStages * kStep + r * kGroup + group] =
+              moves ? page_to[r] * st0 + (i - p.by_page.div(i) * (int)p.by_page.d) * st2 : -1;
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int step = 0; step < kStages - 1; ++step) fetch(step);
+  for (int step = 0; step < n_steps; ++step) {
+    cp_async_wait<kStages - 2>();
+    __syncthreads();  // every row of the step is in shared memory, and every store of the step before has read its rows there
+    fetch(step + kStages - 1);  // (rows at or behind their own new places, which this step and the next do not write)
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const long long at = to[step % kStages * kStep + r * kGroup + group];
+      if (at >= 0) *reinterpret_cast<uint4*>(base + at) = buf[(step % kStages * kRows + r) * kMoveThreads + tid];
+    }
+  }
+  if (bad) atomicOr(p.status, kStatusOutOfRange);
+}
+
+// For few (sequence, KV head) pairs: 32 bytes of a row per CTA, up to 1024 rows a step in registers; the next step's addresses (list
+// entry, then table entry) are on their way while a step's rows arrive.
+__global__ void __launch_bounds__(kMoveThreads) evict_move_few_kernel(const EvictParams p) {
+  constexpr int kLanes = kFewLanes, kRows = 8, kGroup = kMoveThreads / kLanes, kStep = kRows * kGroup;  // kStep: rows a step moves
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int hkv = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, slices = gridDim.x / 2;
   const int n = min(max(p.kv_lens[b], 0), p.max_len);
   if (n <= p.n_keep) return;
   const bool is_v = (int)blockIdx.x >= slices;
@@ -308,11 +382,27 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
   if (bad) atomicOr(p.status, kStatusOutOfRange);
 }
 
-// The columns of a row that one CTA moves: 128 bytes, or 32 where those CTAs would not fill the SMs.
-template <int kLanes>
-cudaError_t launch_move(const EvictParams& p, int batch, int head_dim, cudaStream_t st) {
-  const int slices = head_dim / (8 * kLanes);
-  return launch_overlapped(evict_move_kernel<kLanes>, dim3(2 * slices, p.n_kv_head, batch), dim3(kMoveThreads), 0, st, 1, p, slices);
+// 128 bytes of a row per CTA, or 32 where those CTAs would not fill the SMs.  Both launches of an eviction, 8 KV heads of 128: one
+// sequence of 2049 keys to 1024 11.7 us with the former kernel in columns of 32 bytes, 10.5 with the latter, four of 4096 to
+// 2048 20.9 and 18.0; 64 of 1000 to 500 43.7 and 47.1 (with the latter in columns of 128), 32 of up to 16 K to 4096 152.3 and 154.4.
+int launch_move(const EvictParams& p, int batch, int head_dim, cudaStream_t st) {
+  static std::atomic<bool> set[64] = {};  // per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
+  if (!set[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(evict_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MoveCfg::kSmemBytes);
+    if (e != cudaSuccess) return (int)e;
+    set[dev].store(true, std::memory_order_release);
+  }
+  const int slices = head_dim / (8 * kLanes), few_slices = head_dim / (8 * kFewLanes);
+  if (2ll * slices * p.n_kv_head * batch >= 2ll * sm_count())
+    e = launch_overlapped(evict_move_kernel, dim3(2 * slices, p.n_kv_head, batch), dim3(kMoveThreads), MoveCfg::kSmemBytes, st, 1, p);
+  else
+    e = launch_overlapped(evict_move_few_kernel, dim3(2 * few_slices, p.n_kv_head, batch), dim3(kMoveThreads), 0, st, 1, p);
+  count_launch();
+  return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
 
 cudaError_t allow_clusters_of_16() {
@@ -372,10 +462,7 @@ int launch_paged_evict(const TyrAttnEvictArgs& a, int* status, cudaStream_t st) 
   count_launch();
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
-  const bool wide = 2ll * (a.head_dim / 64) * a.n_kv_head * a.batch >= 2ll * sm_count();
-  e = wide ? launch_move<8>(p, a.batch, a.head_dim, st) : launch_move<2>(p, a.batch, a.head_dim, st);
-  count_launch();
-  return (int)(e != cudaSuccess ? e : cudaGetLastError());
+  return launch_move(p, a.batch, a.head_dim, st);
 }
 
 }  // namespace tyr
