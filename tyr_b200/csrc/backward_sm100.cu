@@ -1117,7 +1117,8 @@ __global__ void __launch_bounds__(256) bwd_sink_merge_kernel(const BwdParams p) 
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int k = 0; k < p.sink_parts; ++k) {
-    const float4 v = *reinterpret_cast<const float4*>(from + k * heads * (2 * kT * D));
+    // (from L2: written by the grid before the one this grid follows)
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(from + k * heads * (2 * kT * D)));
     acc.x += v.x;
     acc.y += v.y;
     acc.z += v.z;

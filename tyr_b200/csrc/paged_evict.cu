@@ -34,7 +34,7 @@ struct EvictParams {
   const int32_t* table;
   int64_t table_stride;
   FastDiv by_page;
-  int n_pages, max_pages;
+  int n_pages;
   const int32_t* kv_lens;
   float* weights;
   int64_t w_stride_b, w_stride_h;
@@ -428,7 +428,6 @@ int launch_paged_evict(const TyrAttnEvictArgs& a, int* status, cudaStream_t st) 
   p.table_stride = a.pages.table_stride;
   p.by_page = make_fastdiv(a.pages.page_size);
   p.n_pages = a.pages.n_pages;
-  p.max_pages = a.pages.max_pages;
   p.kv_lens = a.kv_lens;
   p.weights = a.weights;
   p.w_stride_b = a.weights_stride[0];
