@@ -258,7 +258,7 @@ typedef struct TyrAttnPageTable {
  * sequence's last key.  With window_size > 0 it sees the last window_size keys and the first n_sink
  * ones (0: every key); what it does not see is not read.
  * kv_lens must be in [0, max_kv_seq]: a sequence of length 0 (an idle slot) gets a zero row and LSE = -inf; a
- * length outside is clamped and sets TYR_ATTN_STATUS_OUT_OF_RANGE.  A bad page table entry gives NaN rows.
+ * length outside is clamped and sets TYR_ATTN_STATUS_OUT_OF_RANGE.  A bad page table entry gives NaN rows (and NaN sums of weights).
  * `weights`, when not NULL, is a running sum per (sequence, KV head, key): the call adds, for every visible key, the
  * softmax weights that the query heads of the group gave it; entries of other keys stay as they are.  No atomics: the
  * same bits each time.
@@ -298,7 +298,7 @@ int tyr_b200_attn_paged_decode(const TyrAttnPagedDecodeArgs* args, void* stream)
  * their weights likewise and clears the weights from there to the sequence's old length.  Other rows stay as they
  * are.  A sequence of at most n_keep keys keeps everything in place.  The sequences' pages must be their own: a
  * page that two of them share would be moved under the other.
- * kept[b, h, i] is the old position of key i, -1 behind a sequence's last.  new_lens must not be kv_lens.
+ * kept[b, h, i] is the old position of key i, -1 behind a sequence's last.  new_lens must not overlap kv_lens.
  * A length outside [0, max_kv_seq] is clamped and reported; a row whose page table entry is bad is not moved.
  * Two launches. */
 typedef struct TyrAttnEvictArgs {
@@ -311,7 +311,7 @@ typedef struct TyrAttnEvictArgs {
   int32_t* new_lens;      /* out, DEVICE int32 [batch]: min(length, n_keep) */
   int32_t* kept;          /* out, DEVICE int32 [batch, n_kv_head, n_keep] contiguous */
   int32_t batch, n_kv_head, max_kv_seq, head_dim; /* head_dim in {64,128,256} */
-  int32_t n_keep, n_recent, n_sink; /* n_keep > 0, n_recent + n_sink <= n_keep */
+  int32_t n_keep, n_recent, n_sink; /* 0 < n_keep <= 2^30, n_recent + n_sink <= n_keep */
   int64_t k_stride[3];    /* elements: page, KV head, row; multiples of 8 */
   int64_t v_stride[3];
 } TyrAttnEvictArgs;

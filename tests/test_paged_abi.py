@@ -114,6 +114,12 @@ def test_evict(built_lib, mem):
     assert call(max_kv_seq=65, weights_stride=[256, 128]) == -11
     assert call(k=p + 8) == -4 and call(v_stride=[2048, 1024, 4]) == -4
     assert call(n_kv_head=70000) == -10
+    # (the list of the kept keys is walked in steps of up to 2048 in 32 bits)
+    assert call(n_keep=(1 << 30) + 1) == -10 and call(n_keep=2 ** 31 - 1) == -10
+    assert call(new_lens=p + 4) == -2 and call(kv_lens=p + 4, new_lens=p) == -2         # overlapping lengths
+    # two heads of a page of 16 rows, and two pages, on one another
+    assert call(k_stride=[2048, 64, 64]) == -2 and call(v_stride=[2048, 512, 64]) == -2 and call(k_stride=[1024, 1024, 64]) == -2
+    assert call(v_stride=[1 << 62, 1024, 64]) == -2
     assert call(pages=table(p, max_pages=2, page_size=(1 << 30) - 1), max_kv_seq=(1 << 30) + 1) == -10
 
 
@@ -138,6 +144,7 @@ def test_append(built_lib, mem):
     assert call(pages=table(p, page_size=1 << 29)) == -10
     assert call(out=p + 8) == -4 and call(head_dim=96) == -3
     assert call(out_stride=[2048, 0, 64]) == -2 and call(out_stride=[0, 1024, 64]) == -2      # heads or pages on one another
+    assert call(out_stride=[2048, 64, 64]) == -2 and call(out_stride=[1024, 1024, 64]) == -2
     assert call(cos=p, sin=p) == -2                                  # a rotary table without rows
     assert call(cos=p, sin=p, max_pos=2) == -11
 

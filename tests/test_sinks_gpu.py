@@ -172,3 +172,12 @@ def test_on_the_other_device():
         got.append([x.cpu() for x in (o, lse, *tnn.attentionBwd(q, k, v, o, lse, d_o, window_size=90, n_sink=4))])
     assert torch.cuda.current_device() == 0 and tnn.device_status(1, True) == 0
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("n_sink", [0, 2])
+def test_a_window_past_32_bits_is_all_keys(n_sink):
+    torch.manual_seed(21)
+    q, k, v = (torch.randn(1, 4, 300, 64, device="cuda").bfloat16() for _ in range(3))
+    want = tnn.scaledDotProductAttentionGQAWindowSinks(q, k, v, window_size=300, n_sink=n_sink)
+    for window in (2 ** 31 - 1, 2 ** 32, 2 ** 32 + 5):
+        assert torch.equal(tnn.scaledDotProductAttentionGQAWindowSinks(q, k, v, window_size=window, n_sink=n_sink), want), window

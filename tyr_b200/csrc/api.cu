@@ -11,6 +11,7 @@
 #include <cstring>
 #include <initializer_list>
 #include <mutex>
+#include <utility>
 
 #include "attn_internal.h"
 #include "ptx_sm100.cuh"
@@ -147,9 +148,17 @@ int check_page_table(const TyrAttnPageTable& t, int64_t max_kv_seq) {
 bool pool_aligned(const void* pool, const int64_t* stride) {
   return aligned16(pool) && !((stride[0] | stride[1] | stride[2]) & 7) && stride[2] > 0 && stride[0] >= 0 && stride[1] >= 0;
 }
-// a pool that is written to: no two of its rows overlap along any axis
+// a pool that is written to: no two of its rows overlap (each axis steps over all that the axes inside it cover)
 bool pool_rows_apart(const int64_t* stride, int n_pages, int heads, int page_size, int head_dim) {
-  return (n_pages == 1 || stride[0] >= head_dim) && (heads == 1 || stride[1] >= head_dim) && (page_size == 1 || stride[2] >= head_dim);
+  std::pair<int64_t, int64_t> axis[3] = {{stride[0], n_pages}, {stride[1], heads}, {stride[2], page_size}};
+  std::sort(axis, axis + 3);
+  int64_t covered = head_dim;
+  for (const auto& [step, count] : axis) {
+    if (count == 1) continue;
+    if (step < covered || step > (int64_t{1} << 60) / count) return false;
+    covered += (count - 1) * step;
+  }
+  return true;
 }
 // the (sequence, KV head) rows of the running sums are written by different CTAs: they may not overlap
 bool sums_apart(const int64_t* stride, int64_t batch, int64_t n_kv_head, int64_t max_kv_seq) {
@@ -362,10 +371,13 @@ int tyr_b200_attn_paged_evict(const TyrAttnEvictArgs* a, void* stream) {
   if (a->batch <= 0 || a->n_kv_head <= 0 || a->max_kv_seq <= 0) return -TYR_ATTN_ERR_SHAPE;
   if (a->n_keep <= 0 || a->n_recent < 0 || a->n_sink < 0 || (int64_t)a->n_recent + a->n_sink > a->n_keep) return -TYR_ATTN_ERR_SHAPE;
   if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return -TYR_ATTN_ERR_HEAD_DIM;
-  if (a->batch > 65535 || a->n_kv_head > 65535 || a->max_kv_seq > kMaxPagedKeys) return -TYR_ATTN_ERR_TOO_LARGE;
+  if (a->batch > 65535 || a->n_kv_head > 65535 || a->max_kv_seq > kMaxPagedKeys || a->n_keep > kMaxPagedKeys)
+    return -TYR_ATTN_ERR_TOO_LARGE;
   if (!sums_apart(a->weights_stride, a->batch, a->n_kv_head, a->max_kv_seq)) return -TYR_ATTN_ERR_SHAPE;
   if (a->batch > 1 && a->pages.table_stride == 0) return -TYR_ATTN_ERR_SHAPE;  // one row of the table for all: shared pages
-  if (a->new_lens == a->kv_lens) return -TYR_ATTN_ERR_SHAPE;  // the lengths are read until the last row has moved
+  // the lengths are read until the last row has moved
+  const uintptr_t lens = reinterpret_cast<uintptr_t>(a->kv_lens), out = reinterpret_cast<uintptr_t>(a->new_lens), bytes = sizeof(int32_t) * a->batch;
+  if (out < lens + bytes && lens < out + bytes) return -TYR_ATTN_ERR_SHAPE;
   int rc = check_page_table(a->pages, a->max_kv_seq);
   if (rc) return rc;
   if (!pool_aligned(a->k, a->k_stride) || !pool_aligned(a->v, a->v_stride)) return -TYR_ATTN_ERR_ALIGN;

@@ -184,7 +184,9 @@ def scaledDotProductAttentionGQAWindowSinks(query, key, value, dropout_p: float 
         raise AttnError(-2)
     if query.shape[2] != key.shape[2]:
         raise ValueError("scaledDotProductAttentionGQAWindowSinks needs q_seq == kv_seq")
-    out, _ = attentionFwd(query, key, value, is_causal=True, return_lse=False, window_size=window_size, n_sink=n_sink)
+    # (a window beyond the keys is all of them, also one that does not fit 32 bits)
+    out, _ = attentionFwd(query, key, value, is_causal=True, return_lse=False, window_size=min(window_size, max(key.shape[2], 1)),
+                          n_sink=n_sink)
     return out
 
 
@@ -326,7 +328,7 @@ def flashDecodePaged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     kv_lens int32 [B], the new token's key included.  Row r of a sequence is row r % page_size of page
     page_table[b, r // page_size].  `max_kv_seq` (default: all the table can hold) bounds the lengths.  A sequence of
     length 0 gets zeros and LSE = -inf; a length outside [0, max_kv_seq] is clamped, and it and a used table entry that
-    is no page (NaN rows) set the out-of-range bit of the device status word.
+    is no page (NaN rows, and NaN `weights`) set the out-of-range bit of the device status word.
     `window_size` > 0: only the last `window_size` keys and the first `n_sink` are seen, and read; pages wholly
     between them may be given back.
     `weights` float32 [B, n_kv_head, >= max_kv_seq]: the softmax weights each visible key got from the query heads of
@@ -358,7 +360,7 @@ def evictPaged(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
     lower position, a NaN below every number) stay.  Their K and V rows move, in the order of their positions, to the
     sequence's first `n_keep` rows, in place, and their weights likewise; the weights behind them, up to the old
     length, become 0.  `kept` holds the old positions (-1 behind a sequence's last key), `new_lens` min(length, n_keep);
-    kv_lens itself is not changed and must not be given as new_lens.  Pages behind the new length may be given back.  The
+    kv_lens itself is not changed and must not be given (nor any part of it) as new_lens.  Pages behind the new length may be given back.  The
     sequences may not share pages.
     """
     return _lib.calls().evict_paged(k_pages, v_pages, page_table, kv_lens, weights, n_keep, n_recent, n_sink, max_kv_seq, new_lens,
