@@ -130,11 +130,17 @@ int check_prefill(const TyrAttnPrefillArgs* a) {
   return 0;
 }
 
-// First tokens beside a window.  A window beyond the keys is taken as all of them.
-int check_sinks(int n_sink, int kv_seq, const void* key_mask, int32_t* window) {
-  if (n_sink < 0 || (n_sink > 0 && (*window <= 0 || key_mask))) return -TYR_ATTN_ERR_SHAPE;
-  if (n_sink > 0 && kv_seq > 0) *window = std::min(*window, kv_seq);
-  return 0;
+// First tokens beside a window.
+int check_sinks(int n_sink, int window, const void* key_mask) {
+  return n_sink < 0 || (n_sink > 0 && (window <= 0 || key_mask)) ? -TYR_ATTN_ERR_SHAPE : 0;
+}
+// The arguments with a window no longer than the keys: such a one hides the same keys, and the kernels add it to
+// positions in 32 bits.
+template <class Args>
+Args with_window_of_keys(const Args& a) {
+  Args d = a;
+  if (d.window_size > 0 && d.kv_seq > 0) d.window_size = std::min(d.window_size, d.kv_seq);
+  return d;
 }
 
 // ---- paged cache
@@ -242,10 +248,11 @@ using namespace tyr;
 
 extern "C" {
 
-static int prefill(const TyrAttnPrefillArgs* a, int n_sink, void* stream) {
-  if (const int kind = empty_kind(a)) return kind == 1 ? 0 : launch_no_keys(*a, static_cast<cudaStream_t>(stream));
-  int rc = check_prefill(a);
+static int prefill(const TyrAttnPrefillArgs* args, int n_sink, void* stream) {
+  if (const int kind = empty_kind(args)) return kind == 1 ? 0 : launch_no_keys(*args, static_cast<cudaStream_t>(stream));
+  int rc = check_prefill(args);
   if (rc) return rc;
+  const TyrAttnPrefillArgs clamped = with_window_of_keys(*args), *a = &clamped;
   const float scale = resolve_scale(a->scale, a->head_dim);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (a->check_mode) return launch_prefill_check(*a, n_sink, scale, st);
@@ -261,9 +268,8 @@ int tyr_b200_attn_prefill(const TyrAttnPrefillArgs* a, void* stream) { return pr
 
 int tyr_b200_attn_prefill_sinks(const TyrAttnPrefillArgs* a, int32_t n_sink, void* stream) {
   if (!a) return -TYR_ATTN_ERR_NULL;
-  TyrAttnPrefillArgs d = *a;
-  const int rc = check_sinks(n_sink, a->kv_seq, a->key_mask, &d.window_size);
-  return rc ? rc : prefill(&d, n_sink, stream);
+  const int rc = check_sinks(n_sink, a->window_size, a->key_mask);
+  return rc ? rc : prefill(a, n_sink, stream);
 }
 
 int tyr_b200_sdpa_4d(uint64_t batch, uint64_t n_head, uint64_t seq, uint64_t head_dim, const void* q,
@@ -445,7 +451,8 @@ uint64_t tyr_b200_attn_backward_workspace_bytes(int32_t batch, int32_t n_head, i
   return backward_workspace_bytes(batch, n_head, q_seq);
 }
 
-static int backward(const TyrAttnBackwardArgs* a, int n_sink, void* stream) {
+static int backward(const TyrAttnBackwardArgs* args, int n_sink, void* stream) {
+  const TyrAttnBackwardArgs clamped = args ? with_window_of_keys(*args) : TyrAttnBackwardArgs{}, *a = args ? &clamped : nullptr;
   // Zero extents as autograd of ATen's operator treats them: without queries (or heads, or a batch)
   // dQ has no element and dK, dV are zeros; without keys dK, dV have no element and dQ is zeros.
   if (a && a->batch >= 0 && a->n_head >= 0 && a->n_kv_head >= 0 && a->q_seq >= 0 && a->kv_seq >= 0 &&
@@ -500,21 +507,19 @@ int tyr_b200_attn_backward(const TyrAttnBackwardArgs* a, void* stream) { return 
 
 int tyr_b200_attn_backward_sinks(const TyrAttnBackwardArgs* a, int32_t n_sink, void* stream) {
   if (!a) return -TYR_ATTN_ERR_NULL;
-  TyrAttnBackwardArgs d = *a;
-  const int rc = check_sinks(n_sink, a->kv_seq, a->key_mask, &d.window_size);
-  return rc ? rc : backward(&d, n_sink, stream);
+  const int rc = check_sinks(n_sink, a->window_size, a->key_mask);
+  return rc ? rc : backward(a, n_sink, stream);
 }
 
 int64_t tyr_b200_attn_backward_sinks_workspace_bytes(const TyrAttnBackwardArgs* a, int32_t n_sink) {
   if (!a) return -TYR_ATTN_ERR_NULL;
-  TyrAttnBackwardArgs d = *a;
-  const int rc = check_sinks(n_sink, a->kv_seq, a->key_mask, &d.window_size);
+  const int rc = check_sinks(n_sink, a->window_size, a->key_mask);
   if (rc) return rc;
   if (a->batch < 0 || a->n_head < 0 || a->n_kv_head < 0 || a->q_seq < 0 || a->kv_seq < 0) return -TYR_ATTN_ERR_SHAPE;
   if (a->batch == 0 || a->n_head == 0 || a->n_kv_head == 0 || a->q_seq == 0 || a->kv_seq == 0) return 0;
   if (a->n_head % a->n_kv_head != 0) return -TYR_ATTN_ERR_SHAPE;
   if (a->head_dim != 64 && a->head_dim != 128) return -TYR_ATTN_ERR_HEAD_DIM;
-  return (int64_t)(n_sink > 0 ? backward_sinks_workspace_bytes(d, n_sink) : backward_workspace_bytes(a->batch, a->n_head, a->q_seq));
+  return (int64_t)(n_sink > 0 ? backward_sinks_workspace_bytes(with_window_of_keys(*a), n_sink) : backward_workspace_bytes(a->batch, a->n_head, a->q_seq));
 }
 
 int64_t tyr_b200_attn_prefill_workspace_bytes(const TyrAttnPrefillArgs* a) {
