@@ -10,7 +10,8 @@ from tyr_b200 import nn as tnn
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
-WINDOWS = [2 ** 31 - 1, 2 ** 31 - 100, 2 ** 30 + 1]
+# near and past 31 bits, past 32 (5 and 0 in the low bits), past what a C int could be cut down from
+WINDOWS = [2 ** 31 - 1, 2 ** 31 - 100, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 40 + 1]
 
 
 def randn(*shape, seed):
@@ -55,6 +56,19 @@ def test_typed_call():
     want = tnn.scaledDotProductAttentionGQAWindow(q, k, v, window_size=300)
     for window in WINDOWS:
         assert torch.equal(tnn.scaledDotProductAttentionGQAWindow(q, k, v, window_size=window), want), window
+    for bad in (0, -1, -2 ** 31, -2 ** 32, -2 ** 32 + 5):
+        with pytest.raises(tnn.AttnError):
+            tnn.scaledDotProductAttentionGQAWindow(q, k, v, window_size=bad)
+
+
+def test_negative_windows_are_refused():
+    q, k, v, d_o = (randn(1, 2, 64, 64, seed=i) for i in range(4))
+    o, lse = tnn.attentionFwd(q, k, v)
+    for bad in (-1, -2 ** 31, -2 ** 32, -2 ** 32 + 5):
+        with pytest.raises(tnn.AttnError):
+            tnn.attentionFwd(q, k, v, window_size=bad)
+        with pytest.raises(tnn.AttnError):
+            tnn.attentionBwd(q, k, v, o, lse, d_o, window_size=bad)
 
 
 def test_c_abi_with_the_greatest_window():

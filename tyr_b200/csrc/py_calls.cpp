@@ -169,7 +169,7 @@ PyObject* attention_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.scale = scale_of(args[4]);
     a.check_mode = check_mode;
     const int32_t n_sink = span_of(args[12]);
-    a.window_size = n_sink != 0 ? span_of(args[9]) : i32(integer(args[9]));
+    a.window_size = span_of(args[9]);
     if (lse_in && (lse_in->scalar_type() != at::kFloat || !lse_in->is_contiguous() || lse_in->dim() != 3 ||
                    lse_in->size(0) != q.size(0) || lse_in->size(1) != q.size(1) || lse_in->size(2) != q.size(2)))
       throw ValueError("lse must be a contiguous float32 [batch, n_head, q_seq] tensor");
@@ -248,7 +248,7 @@ PyObject* attention_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.is_causal = truth(args[6]);
     a.scale = scale_of(args[7]);
     const int32_t n_sink = span_of(args[11]);
-    a.window_size = n_sink != 0 ? span_of(args[9]) : i32(integer(args[9]));
+    a.window_size = span_of(args[9]);
     if (mask) {
       const Tensor m = key_bytes(*mask, k.size(0), k.size(2));
       a.key_mask = static_cast<const uint8_t*>(m.data_ptr());
