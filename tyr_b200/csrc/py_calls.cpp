@@ -480,12 +480,13 @@ PyObject* paged_decode_call(PyObject* const* args, Py_ssize_t n, bool only_bytes
   const Tensor *w = maybe(args[8], "weights"), *out_in = maybe(args[10], "out"), *lse_in = maybe(args[11], "lse"),
                *ws_in = maybe(args[12], "workspace");
   const int64_t cap = (int64_t)a.pages.max_pages * a.pages.page_size;
-  a.max_kv_seq = count_of(args[5] == Py_None ? (w && w->dim() == 3 && w->size(2) < cap ? w->size(2) : cap) : integer(args[5]), "max_kv_seq");
+  a.max_kv_seq = count_of(args[5] == Py_None ? cap : integer(args[5]), "max_kv_seq");
   a.window_size = span_of(args[6]);
   a.n_sink = span_of(args[7]);
   if (w) {
     a.weights = weight_sums(*w, q, r.batch, k.size(1), a.weights_stride);
-    if (w->size(2) < a.max_kv_seq) throw ValueError("weights holds fewer keys than max_kv_seq");
+    if (w->size(2) < a.max_kv_seq)
+      throw ValueError("weights holds fewer keys than max_kv_seq (where it is not given, all the page table can hold)");
   }
   a.scale = scale_of(args[9]);
   const bool return_lse = truth(args[13]);

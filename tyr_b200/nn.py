@@ -326,7 +326,7 @@ def flashDecodePaged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     q [B, n_head, head_dim] (or [B, n_head, 1, head_dim]) bf16; k_pages, v_pages [n_pages, n_kv_head, page_size,
     head_dim] bf16, views of any order of those axes with unit stride on the last; page_table int32 [B, max_pages];
     kv_lens int32 [B], the new token's key included.  Row r of a sequence is row r % page_size of page
-    page_table[b, r // page_size].  `max_kv_seq` (default: all the table can hold) bounds the lengths.  A sequence of
+    page_table[b, r // page_size].  `max_kv_seq` (default: all the table can hold, with or without `weights`) bounds the lengths.  A sequence of
     length 0 gets zeros and LSE = -inf; a length outside [0, max_kv_seq] is clamped, and it and a used table entry that
     is no page (NaN rows, and NaN `weights`) set the out-of-range bit of the device status word.
     `window_size` > 0: only the last `window_size` keys and the first `n_sink` are seen, and read; pages wholly
@@ -336,6 +336,7 @@ def flashDecodePaged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     `total_kv_len`: the sum of the lengths where the host knows it (it steers how the launch is cut).
     `workspace`: a caller-kept uint8 tensor of `paged_decode_workspace_bytes(...)` bytes, 16-byte aligned, for one call at a
     time (calls on two streams, or two captured graphs that may run at once, need one each); allocated otherwise.
+    With `weights` it holds every score: 4 bytes for each sequence, query head and key that max_kv_seq lets it see.
     """
     return _lib.calls().decode_paged(q, k_pages, v_pages, page_table, kv_lens, max_kv_seq, window_size, n_sink, weights, scale,
                                      out, lse, workspace, return_lse, total_kv_len, max_splits)
@@ -361,7 +362,8 @@ def evictPaged(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
     sequence's first `n_keep` rows, in place, and their weights likewise; the weights behind them, up to the old
     length, become 0.  `kept` holds the old positions (-1 behind a sequence's last key), `new_lens` min(length, n_keep);
     kv_lens itself is not changed and must not be given (nor any part of it) as new_lens.  Pages behind the new length may be given back.  The
-    sequences may not share pages.
+    sequences may not share pages.  `max_kv_seq` (default: what the table and `weights` can both hold) bounds the lengths; a
+    length outside [0, max_kv_seq] is clamped and sets the out-of-range bit of the device status word.
     """
     return _lib.calls().evict_paged(k_pages, v_pages, page_table, kv_lens, weights, n_keep, n_recent, n_sink, max_kv_seq, new_lens,
                                     kept)
