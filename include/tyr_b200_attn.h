@@ -298,6 +298,8 @@ int tyr_b200_attn_paged_decode(const TyrAttnPagedDecodeArgs* args, void* stream)
  * their weights likewise and clears the weights from there to the sequence's old length.  Other rows stay as they
  * are.  A sequence of at most n_keep keys keeps everything in place.  The sequences' pages must be their own: a
  * page that two of them share would be moved under the other.
+ * K and V are moved side by side: no row of one pool may share memory with a row of the other (-TYR_ATTN_ERR_SHAPE, also where
+ * the pools lie in one another but are laid out differently there; K and V interleaved in one allocation are fine).
  * kept[b, h, i] is the old position of key i, -1 behind a sequence's last.  new_lens must not overlap kv_lens.
  * A length outside [0, max_kv_seq] is clamped and reported; a row whose page table entry is bad is not moved.
  * Two launches. */

@@ -9,6 +9,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstring>
+#include <functional>
 #include <initializer_list>
 #include <mutex>
 #include <utility>
@@ -165,6 +166,32 @@ bool pool_rows_apart(const int64_t* stride, int n_pages, int heads, int page_siz
     covered += (count - 1) * step;
   }
   return true;
+}
+// Two pools whose rows are written by different CTAs, K's and V's of an eviction: no row of one shares memory with a row of
+// the other.  Both have passed the check above, so a pool is nested blocks, outermost axis first, each of which steps over all that is
+// inside it.  Blocks whose spans do not meet are apart; where the outer axes of both step alike only neighbouring blocks
+// can meet, and those are looked into.  Blocks that meet but are laid out differently count as overlapping.
+struct PoolAxes {
+  std::pair<int64_t, int64_t> axis[3];  // step, count; greatest step first
+  int64_t span[4];                      // elements from the first to behind the last of what lies inside axis i, i + 1, ..
+  PoolAxes(const int64_t* stride, int n_pages, int heads, int page_size, int head_dim)
+      : axis{{stride[0], n_pages}, {stride[1], heads}, {stride[2], page_size}} {
+    for (auto& x : axis)
+      if (x.second == 1) x.first = 0;   // never stepped over
+    std::sort(axis, axis + 3, std::greater<>());
+    span[3] = head_dim;
+    for (int i = 2; i >= 0; --i) span[i] = span[i + 1] + (axis[i].second - 1) * axis[i].first;
+  }
+};
+bool pools_meet(const PoolAxes& a, const PoolAxes& b, int64_t ahead, int i = 0) {  // b's block begins `ahead` elements behind a's
+  if (ahead >= a.span[i] || -ahead >= b.span[i]) return false;
+  if (i == 3 || a.axis[i] != b.axis[i]) return true;
+  const auto [step, count] = a.axis[i];
+  if (step == 0) return pools_meet(a, b, ahead, i + 1);
+  const int64_t near = -ahead / step;
+  for (int64_t d = std::max(near - 1, 1 - count); d <= std::min(near + 1, count - 1); ++d)
+    if (pools_meet(a, b, ahead + d * step, i + 1)) return true;
+  return false;
 }
 // the (sequence, KV head) rows of the running sums are written by different CTAs: they may not overlap
 bool sums_apart(const int64_t* stride, int64_t batch, int64_t n_kv_head, int64_t max_kv_seq) {
@@ -389,6 +416,11 @@ int tyr_b200_attn_paged_evict(const TyrAttnEvictArgs* a, void* stream) {
   if (!pool_aligned(a->k, a->k_stride) || !pool_aligned(a->v, a->v_stride)) return -TYR_ATTN_ERR_ALIGN;
   for (const int64_t* st : {a->k_stride, a->v_stride})
     if (!pool_rows_apart(st, a->pages.n_pages, a->n_kv_head, a->pages.page_size, a->head_dim)) return -TYR_ATTN_ERR_SHAPE;
+  {
+    auto axes = [&](const int64_t* st) { return PoolAxes(st, a->pages.n_pages, a->n_kv_head, a->pages.page_size, a->head_dim); };
+    const int64_t ahead = (reinterpret_cast<intptr_t>(a->v) - reinterpret_cast<intptr_t>(a->k)) / 2;  // (both 16-byte aligned)
+    if (pools_meet(axes(a->k_stride), axes(a->v_stride), ahead)) return -TYR_ATTN_ERR_SHAPE;
+  }
   if (reinterpret_cast<uintptr_t>(a->weights) & 3u) return -TYR_ATTN_ERR_ALIGN;
   int dev = 0;
   if ((rc = current_device_checked(&dev))) return rc;

@@ -362,7 +362,7 @@ def evictPaged(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
     sequence's first `n_keep` rows, in place, and their weights likewise; the weights behind them, up to the old
     length, become 0.  `kept` holds the old positions (-1 behind a sequence's last key), `new_lens` min(length, n_keep);
     kv_lens itself is not changed and must not be given (nor any part of it) as new_lens.  Pages behind the new length may be given back.  The
-    sequences may not share pages.  `max_kv_seq` (default: what the table and `weights` can both hold) bounds the lengths; a
+    sequences may not share pages, nor K and V rows.  `max_kv_seq` (default: what the table and `weights` can both hold) bounds the lengths; a
     length outside [0, max_kv_seq] is clamped and sets the out-of-range bit of the device status word.
     """
     return _lib.calls().evict_paged(k_pages, v_pages, page_table, kv_lens, weights, n_keep, n_recent, n_sink, max_kv_seq, new_lens,
