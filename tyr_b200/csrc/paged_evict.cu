@@ -20,6 +20,7 @@
 #include <atomic>
 
 #include "attn_internal.h"
+#include "evict_plan.h"
 #include "fast_div.h"
 #include "mma_sync.cuh"
 #include "ptx_sm100.cuh"
@@ -54,7 +55,6 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 
 // Positions a thread holds at once: position k * kThreads + thread as item k.
 constexpr int kItems = 16, kAhead = 4;
-constexpr int kMaxCluster = 16;
 // kCluster: the CTAs of a cluster share the (sequence, KV head), a segment of kItems * kThreads positions each, so that a
 // long sequence's weights stay in registers too; the histograms and counts are added through distributed shared memory.
 // Otherwise one CTA, which reads the weights again in every pass where they are more than a segment.
@@ -405,17 +405,30 @@ int launch_move(const EvictParams& p, int batch, int head_dim, cudaStream_t st) 
   return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
 
-cudaError_t allow_clusters_of_16() {
-  static std::atomic<bool> set[64] = {};  // per device
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!set[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(evict_select_kernel<1024, true, 11>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess) set[dev].store(true, std::memory_order_release);
+// Clusters of 2^k CTAs of the selection that can be resident at once: depends on how the SMs are spread over the GPCs, asked for
+// once per device.
+int cluster_capacity(int dev, int k) {
+  static std::atomic<int> known[64][kMaxEvictLog + 1] = {};  // per device; 0: not asked yet, else capacity + 1
+  const int have = known[dev][k].load(std::memory_order_acquire);
+  if (have > 0) return have - 1;
+  auto* kernel = evict_select_kernel<1024, true, 11>;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 1u << k;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1u << k);
+  cfg.blockDim = dim3(1024);
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();  // no clusters of this size then
+    n = 0;
   }
-  return e;
+  known[dev][k].store(n + 1, std::memory_order_release);
+  return n;
 }
 
 }  // namespace
@@ -441,18 +454,17 @@ int launch_paged_evict(const TyrAttnEvictArgs& a, int* status, cudaStream_t st) 
   p.n_sink = a.n_sink;
   for (int i = 0; i < 3; ++i) { p.ks[i] = a.k_stride[i]; p.vs[i] = a.v_stride[i]; }
   p.status = status;
-  // Half as many threads, two CTAs per SM, while they hold a sequence: 64 sequences of 1000 keys, 8 KV heads, both launches
-  // 56.9 -> 47.0 us, one of 2049 11.1 -> 10.5; with half as many for 32 sequences of up to 16 K 155.8 -> 161.9.  Digits of 11 bits
-  // there: one of 2049 11.2 us.  Past what one CTA holds a cluster, up to 16 times as much (one sequence of 30000 keys 50.0 ->
-  // 37.5 us, of 100000 the first launch alone 97 -> 28); what is longer still is one CTA's, in segments.
+  // Half as many threads, two CTAs per SM, while they hold a sequence (both launches, every pass with new weights: 64 sequences of 1000
+  // keys, 8 KV heads of 128, 85 -> 73 us; for 32 sequences of up to 16 K half as many take 261 for 237), and digits of 8 bits there
+  // (64 of 1000 with digits of 11 75).
   const int segment = kItems * 1024;
   const bool few = a.max_kv_seq <= kItems * 512;
-  p.ranks = 1;
-  while (p.ranks < kMaxCluster && (long long)p.ranks * segment < a.max_kv_seq) p.ranks *= 2;
-  if ((long long)p.ranks * segment < a.max_kv_seq) p.ranks = 1;
+  int dev = 0;
+  if (cudaError_t got = cudaGetDevice(&dev); got != cudaSuccess) return (int)got;
+  if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
+  p.ranks = evict_ranks(a.max_kv_seq, segment, [&](int k) { return cluster_capacity(dev, k); });
   cudaError_t e;
   if (p.ranks > 1) {
-    if ((e = allow_clusters_of_16()) != cudaSuccess) return (int)e;
     e = launch_overlapped(evict_select_kernel<1024, true, 11>, dim3(a.n_kv_head * p.ranks, a.batch), dim3(1024), 0, st, p.ranks, p);
   } else {
     e = launch_overlapped(few ? evict_select_kernel<512, false, 8> : evict_select_kernel<1024, false, 11>, dim3(a.n_kv_head, a.batch),
