@@ -96,6 +96,10 @@ void require_cuda(const Tensor& t) {
   if (t.dim() > 4) throw ValueError("tensor rank must be <= 4");
   if (t.dim() < 1 || t.stride(-1) != 1) throw ValueError("tensor must have unit stride on the head dimension");
 }
+// the kernels follow pointers of one device
+void same_device(const Tensor& t, const Tensor& as, const char* what) {
+  if (!t.is_cuda() || t.device() != as.device()) throw ValueError(std::string(what) + " must be on the device of the other tensors");
+}
 void require_count(Py_ssize_t n, Py_ssize_t want) {
   if (n != want) throw ValueError("wrong number of arguments");
 }
@@ -165,6 +169,11 @@ PyObject* attention_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     TyrAttnPrefillArgs a;
     fill_prefill(a, q, k, v, out_in);
     if (out_in) require_cuda(*out_in);
+    same_device(k, q, "k");
+    same_device(v, q, "v");
+    if (out_in) same_device(*out_in, q, "out");
+    if (lse_in) same_device(*lse_in, q, "lse");
+    if (mask) same_device(*mask, q, "key_mask");
     a.is_causal = causal;
     a.scale = scale_of(args[4]);
     a.check_mode = check_mode;
@@ -236,6 +245,9 @@ PyObject* attention_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (lse.scalar_type() != at::kFloat || !lse.is_contiguous())
       throw ValueError("lse must be a contiguous float32 [batch, n_head, q_seq] tensor");
     const Tensor *ws_in = maybe(args[8], "workspace"), *mask = maybe(args[10], "key_mask");
+    for (const Tensor* t : {&k, &v, &o, &lse, &d_o}) same_device(*t, q, "k, v, o, lse and d_o");
+    if (ws_in) same_device(*ws_in, q, "workspace");
+    if (mask) same_device(*mask, q, "key_mask");
     TyrAttnBackwardArgs a;
     std::memset(&a, 0, sizeof(a));
     a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr(); a.o = o.data_ptr(); a.d_o = d_o.data_ptr();
@@ -332,6 +344,10 @@ PyObject* decode_ragged(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.scale = scale_of(args[14]);
     const Tensor *out_in = maybe(args[15], "out"), *lse_in = maybe(args[16], "lse");
     const bool return_lse = truth(args[17]);
+    same_device(tensor(args[8], "k_ptrs"), q, "the plan's arrays");
+    if (ws) same_device(*ws, q, "the plan's workspace");
+    if (out_in) same_device(*out_in, q, "out");
+    if (lse_in) same_device(*lse_in, q, "lse");
     a.q = q.data_ptr();
     a.q_stride[0] = r.stride_b;
     a.q_stride[1] = r.stride_h;
@@ -363,6 +379,10 @@ PyObject* decode_dense(PyObject*, PyObject* const* args, Py_ssize_t n) {
     require_cuda(v);
     if (k.dim() != 4 || v.dim() != 4) throw ValueError("k_cache and v_cache must be [batch, n_kv_head, cap, head_dim]");
     const Tensor *lens = maybe(args[3], "kv_lens"), *ws_in = maybe(args[6], "workspace");
+    same_device(k, q, "k_cache");
+    same_device(v, q, "v_cache");
+    if (lens) same_device(*lens, q, "kv_lens");
+    if (ws_in) same_device(*ws_in, q, "workspace");
     TyrAttnDecodeArgs a;
     std::memset(&a, 0, sizeof(a));
     a.q = q.data_ptr();
@@ -410,9 +430,6 @@ PyObject* decode_dense(PyObject*, PyObject* const* args, Py_ssize_t n) {
 int32_t count_of(int64_t v, const char* what) {
   if (v < INT32_MIN || v > INT32_MAX) throw ValueError(std::string(what) + " does not fit 32 bits");
   return static_cast<int32_t>(v);
-}
-void same_device(const Tensor& t, const Tensor& as, const char* what) {
-  if (!t.is_cuda() || t.device() != as.device()) throw ValueError(std::string(what) + " must be on the device of the other tensors");
 }
 // int32 [batch], contiguous
 const int32_t* per_sequence(const Tensor& t, const Tensor& as, int64_t batch, const char* what) {
