@@ -383,6 +383,14 @@ PyObject* decode_dense(PyObject*, PyObject* const* args, Py_ssize_t n) {
     same_device(v, q, "v_cache");
     if (lens) same_device(*lens, q, "kv_lens");
     if (ws_in) same_device(*ws_in, q, "workspace");
+    const int64_t kv_len = args[4] == Py_None ? k.size(2) : integer(args[4]);
+    for (const Tensor* t : {&k, &v}) {  // a larger cache than the call needs is fine
+      if (t->scalar_type() != at::kBFloat16 || q.scalar_type() != at::kBFloat16) throw ValueError("q and the caches must be bf16");
+      if (t->size(0) < r.batch || t->size(1) != k.size(1) || t->size(3) != r.d) throw ValueError("the caches do not match q");
+      if (t->size(2) < kv_len) throw ValueError("kv_len " + std::to_string(kv_len) + " exceeds the " + std::to_string(t->size(2)) + " rows of the cache");
+    }
+    if (lens && (lens->scalar_type() != at::kInt || !lens->is_contiguous() || lens->numel() < r.batch))
+      throw ValueError("kv_lens must be a contiguous int32 tensor [batch]");
     TyrAttnDecodeArgs a;
     std::memset(&a, 0, sizeof(a));
     a.q = q.data_ptr();
@@ -392,7 +400,7 @@ PyObject* decode_dense(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.batch = i32(r.batch);
     a.n_head = i32(r.heads);
     a.n_kv_head = i32(k.size(1));
-    a.max_kv_seq = i32(args[4] == Py_None ? k.size(2) : integer(args[4]));
+    a.max_kv_seq = kv_len < 0 ? -1 : i32(kv_len);
     a.head_dim = i32(r.d);
     a.q_stride[0] = r.stride_b;
     a.q_stride[1] = r.stride_h;
