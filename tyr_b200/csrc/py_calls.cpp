@@ -636,17 +636,20 @@ PyObject* qk_prologue(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (rows && !table) throw ValueError("rows goes with page_table");
     if (table) {
       fill_pages(pages, *table, out, B);
-      same_device(out, x, "out");
       if (rows) per_sequence(*rows, x, B, "rows");
-      // (dense calls leave the length of positions to the caller)
       if (args[5] != Py_None) per_sequence(tensor(args[5], "positions"), x, B, "positions");
     }
     const int64_t cap = table ? (int64_t)pages.max_pages * pages.page_size : out.size(2);
     const Tensor *w = maybe(args[2], "norm_weight"), *cos = maybe(args[3], "cos"), *sin = maybe(args[4], "sin"),
                  *pos = maybe(args[5], "positions"), *pe = maybe(args[8], "pe");
-    for (const Tensor* t : {w, cos, sin, pe})
-      if (t && (t->scalar_type() != at::kFloat || !t->is_contiguous() || !t->is_cuda()))
+    for (const Tensor* t : {w, cos, sin, pe}) {
+      if (!t) continue;
+      if (t->scalar_type() != at::kFloat || !t->is_contiguous() || !t->is_cuda())
         throw ValueError("norm_weight / cos / sin / pe must be contiguous float32 CUDA tensors");
+      same_device(*t, x, "norm_weight / cos / sin / pe");
+    }
+    if (w && w->numel() < D) throw ValueError("norm_weight must have head_dim elements");
+    same_device(out, x, "out");
     if (pe) {
       if (cos || sin) throw ValueError("pass either cos/sin or pe");
       if (pe->dim() != 5 || pe->size(2) != D / 2 || pe->size(3) != 2 || pe->size(4) != 2 ||
@@ -667,8 +670,10 @@ PyObject* qk_prologue(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (max_pos && position0 + S > max_pos)
         throw ValueError("positions up to " + std::to_string(position0 + S - 1) + " exceed the " + std::to_string(max_pos) +
                          " rows of the rotary table");
-    } else if (pos->scalar_type() != at::kInt || !pos->is_cuda()) {
-      throw ValueError("positions must be an int32 CUDA tensor");
+    } else {
+      if (pos->scalar_type() != at::kInt || !pos->is_cuda()) throw ValueError("positions must be an int32 CUDA tensor");
+      same_device(*pos, x, "positions");
+      if (pos->numel() < B || !pos->is_contiguous()) throw ValueError("positions must have an element for each sequence");
     }
     TyrAttnPrologueArgs a;
     std::memset(&a, 0, sizeof(a));
