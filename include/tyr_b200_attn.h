@@ -265,7 +265,7 @@ typedef struct TyrAttnPageTable {
  * At most two launches. */
 typedef struct TyrAttnPagedDecodeArgs {
   const void* q; /* [batch, n_head, head_dim] */
-  void* o;       /* [batch, n_head, head_dim] */
+  void* o;       /* [batch, n_head, head_dim]; its rows may not overlap */
   float* lse;    /* [batch, n_head] or NULL */
   const void* k; /* pools, 16-byte aligned */
   const void* v;

@@ -155,7 +155,7 @@ int check_page_table(const TyrAttnPageTable& t, int64_t max_kv_seq) {
 bool pool_aligned(const void* pool, const int64_t* stride) {
   return aligned16(pool) && !((stride[0] | stride[1] | stride[2]) & 7) && stride[2] > 0 && stride[0] >= 0 && stride[1] >= 0;
 }
-// a pool that is written to: no two of its rows overlap (each axis steps over all that the axes inside it cover)
+// an output, or a pool that is written to: no two of its rows overlap (each axis steps over all that the axes inside it cover)
 bool pool_rows_apart(const int64_t* stride, int n_pages, int heads, int page_size, int head_dim) {
   std::pair<int64_t, int64_t> axis[3] = {{stride[0], n_pages}, {stride[1], heads}, {stride[2], page_size}};
   std::sort(axis, axis + 3);
@@ -387,6 +387,8 @@ int tyr_b200_attn_paged_decode(const TyrAttnPagedDecodeArgs* a, void* stream) {
   if ((reinterpret_cast<uintptr_t>(a->q) & 3u) || (a->q_stride[0] & 1) || (a->q_stride[1] & 1) ||
       (reinterpret_cast<uintptr_t>(a->o) & 1u))
     return -TYR_ATTN_ERR_ALIGN;
+  const int64_t o_stride[3] = {a->o_stride[0], a->o_stride[1], a->head_dim};
+  if (!pool_rows_apart(o_stride, a->batch, a->n_head, 1, a->head_dim)) return -TYR_ATTN_ERR_SHAPE;  // written by different CTAs
   if (a->weights && !sums_apart(a->weights_stride, a->batch, a->n_kv_head, a->max_kv_seq)) return -TYR_ATTN_ERR_SHAPE;
   if (a->weights && (reinterpret_cast<uintptr_t>(a->weights) & 3u)) return -TYR_ATTN_ERR_ALIGN;
   const size_t need = paged_decode_workspace_bytes(*a);
