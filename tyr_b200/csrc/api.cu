@@ -40,6 +40,7 @@ struct HostStage {  // device staging buffers of the host-buffer call, grown on 
 HostStage g_stage[kMaxDevices];
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }  // numbers of 32 bits
 
 // scale <= 0 (or NaN) selects ATen's default 1/sqrt(head_dim); the kernels take the row maximum
 // of the raw scores before scaling, which is only valid for a positive scale
@@ -147,6 +148,7 @@ Args with_window_of_keys(const Args& a) {
 // ---- paged cache
 int check_page_table(const TyrAttnPageTable& t, int64_t max_kv_seq) {
   if (t.max_pages <= 0 || t.n_pages <= 0 || t.page_size <= 0 || t.table_stride < 0) return -TYR_ATTN_ERR_SHAPE;
+  if (!aligned4(t.table)) return -TYR_ATTN_ERR_ALIGN;
   const int64_t cap = (int64_t)t.max_pages * t.page_size;
   if (cap > 0x7fffffffLL) return -TYR_ATTN_ERR_TOO_LARGE;
   return max_kv_seq > cap ? -TYR_ATTN_ERR_RANGE : 0;  // a sequence may not reach behind its row of the table
@@ -385,12 +387,12 @@ int tyr_b200_attn_paged_decode(const TyrAttnPagedDecodeArgs* a, void* stream) {
   if ((rc = check_page_table(a->pages, a->max_kv_seq))) return rc;
   if (!pool_aligned(a->k, a->k_stride) || !pool_aligned(a->v, a->v_stride)) return -TYR_ATTN_ERR_ALIGN;
   if ((reinterpret_cast<uintptr_t>(a->q) & 3u) || (a->q_stride[0] & 1) || (a->q_stride[1] & 1) ||
-      (reinterpret_cast<uintptr_t>(a->o) & 1u))
+      (reinterpret_cast<uintptr_t>(a->o) & 1u) || !aligned4(a->kv_lens) || !aligned4(a->lse))
     return -TYR_ATTN_ERR_ALIGN;
   const int64_t o_stride[3] = {a->o_stride[0], a->o_stride[1], a->head_dim};
   if (!pool_rows_apart(o_stride, a->batch, a->n_head, 1, a->head_dim)) return -TYR_ATTN_ERR_SHAPE;  // written by different CTAs
   if (a->weights && !sums_apart(a->weights_stride, a->batch, a->n_kv_head, a->max_kv_seq)) return -TYR_ATTN_ERR_SHAPE;
-  if (a->weights && (reinterpret_cast<uintptr_t>(a->weights) & 3u)) return -TYR_ATTN_ERR_ALIGN;
+  if (!aligned4(a->weights)) return -TYR_ATTN_ERR_ALIGN;
   const size_t need = paged_decode_workspace_bytes(*a);
   if (need > 0 && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < (int64_t)need)) return -TYR_ATTN_ERR_WORKSPACE;
   int dev = 0;
@@ -423,7 +425,9 @@ int tyr_b200_attn_paged_evict(const TyrAttnEvictArgs* a, void* stream) {
     const int64_t ahead = (reinterpret_cast<intptr_t>(a->v) - reinterpret_cast<intptr_t>(a->k)) / 2;  // (both 16-byte aligned)
     if (pools_meet(axes(a->k_stride), axes(a->v_stride), ahead)) return -TYR_ATTN_ERR_SHAPE;
   }
-  if (reinterpret_cast<uintptr_t>(a->weights) & 3u) return -TYR_ATTN_ERR_ALIGN;
+  for (const void* x : {static_cast<const void*>(a->weights), static_cast<const void*>(a->kv_lens), static_cast<const void*>(a->new_lens),
+                        static_cast<const void*>(a->kept)})
+    if (!aligned4(x)) return -TYR_ATTN_ERR_ALIGN;
   int dev = 0;
   if ((rc = current_device_checked(&dev))) return rc;
   DeviceState* ds = device_state(dev);
@@ -466,6 +470,7 @@ static int qk_prologue(const TyrAttnPrologueArgs* a, const TyrAttnPageTable* pag
   for (int i = 0; i < 3; ++i)
     if ((a->x_stride[i] & 7) || (a->out_stride[i] & 7)) return -TYR_ATTN_ERR_ALIGN;
   if (a->pe && (a->pe_batch_stride & 3)) return -TYR_ATTN_ERR_ALIGN;
+  if (!aligned4(rows) || (pages && !aligned4(a->positions))) return -TYR_ATTN_ERR_ALIGN;
   int dev = 0, rc;
   if ((rc = current_device_checked(&dev))) return rc;
   DeviceState* ds = device_state(dev);
