@@ -27,6 +27,8 @@
 extern "C" {
 #endif
 
+/* Changes whenever an existing call or structure does.  Calls that came without touching those leave it as it is (first tokens, the
+ * paged cache and the eviction came at 8): a caller that opens the library at run time finds out about one by its symbol. */
 #define TYR_ATTN_ABI_VERSION 8
 
 /* element types of Q/K/V/O */
