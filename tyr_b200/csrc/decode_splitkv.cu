@@ -251,7 +251,6 @@ decode_kernel(const __grid_constant__ P p) {
   // ---- stage loader: kTileKeys keys x D bf16 of K and of V, 16 bytes per cp.async
   auto load_tile = [&](int tile, int stage, Where where) {
     const uint32_t sk = sbase + stage * C::kStageBytes, sv = sk + C::kTileBytes;
-    const int k0 = key_begin + tile * kTileKeys;
     if constexpr (kPaged) {
       if ((unsigned)where.page >= (unsigned)p.n_pages) {  // not followed
         bad_page = true;
@@ -275,15 +274,16 @@ decode_kernel(const __grid_constant__ P p) {
           cp_async16(sv + sw_off<D>(kr0 + it, c), vbase + c * 8 + __shfl_sync(0xffffffffu, at_v, it, C::kChunksPerRow));
         }
       }
-      return;
-    }
+    } else {
+      const int k0 = key_begin + tile * kTileKeys;
 #pragma unroll
-    for (int it = 0; it < kLoads; ++it) {
-      const int idx = it * kThreads + tid;
-      const int kr = idx / C::kChunksPerRow, c = idx % C::kChunksPerRow;
-      const int key = min(k0 + kr, key_end - 1);  // rows past the end re-read the last valid key
-      cp_async16(sk + sw_off<D>(kr, c), kbase + (int64_t)key * p.ks[2] + c * 8);
-      cp_async16(sv + sw_off<D>(kr, c), vbase + (int64_t)key * p.vs[2] + c * 8);
+      for (int it = 0; it < kLoads; ++it) {
+        const int idx = it * kThreads + tid;
+        const int kr = idx / C::kChunksPerRow, c = idx % C::kChunksPerRow;
+        const int key = min(k0 + kr, key_end - 1);  // rows past the end re-read the last valid key
+        cp_async16(sk + sw_off<D>(kr, c), kbase + (int64_t)key * p.ks[2] + c * 8);
+        cp_async16(sv + sw_off<D>(kr, c), vbase + (int64_t)key * p.vs[2] + c * 8);
+      }
     }
   };
 
