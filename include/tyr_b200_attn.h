@@ -289,7 +289,7 @@ typedef struct TyrAttnPagedDecodeArgs {
 } TyrAttnPagedDecodeArgs;
 
 /* Bytes of workspace the call below needs at most (0: none); looks at sizes, window_size, n_sink, max_splits and at
- * whether `weights` is given.  Negative TYR_ATTN_ERR_* on bad sizes. */
+ * whether `weights` is given (4 bytes then for each sequence, query head and key that max_kv_seq lets it see).  Negative TYR_ATTN_ERR_* on bad sizes. */
 int64_t tyr_b200_attn_paged_decode_workspace_bytes(const TyrAttnPagedDecodeArgs* args);
 int tyr_b200_attn_paged_decode(const TyrAttnPagedDecodeArgs* args, void* stream);
 
@@ -443,7 +443,8 @@ int tyr_b200_attn_backward(const TyrAttnBackwardArgs* args, void* stream);
 
 /* Gradients of tyr_b200_attn_prefill_sinks, with its rules for n_sink; n_sink = 0 is the call above.  The first keys are
  * seen by every query, so where that would leave them to few SMs their query rows are shared out and the partial
- * sums, in the workspace, added in a fixed order by a fourth launch.  workspace: 16-byte aligned, of the size the
+ * sums, in the workspace, added in a fixed order by a fourth launch.  How they are shared out goes by one sequence's sizes, so the
+ * workspace grows with the batch (a first key block's dK and dV in fp32 for each share).  workspace: 16-byte aligned, of the size the
  * function says (at least that of the call above; negative TYR_ATTN_ERR_* on bad arguments). */
 int64_t tyr_b200_attn_backward_sinks_workspace_bytes(const TyrAttnBackwardArgs* args, int32_t n_sink);
 int tyr_b200_attn_backward_sinks(const TyrAttnBackwardArgs* args, int32_t n_sink, void* stream);

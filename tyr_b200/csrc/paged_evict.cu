@@ -1,9 +1,11 @@
 // Eviction from a paged KV cache by accumulated attention weight: per (sequence, KV head) the first n_sink and the last
 // n_recent keys stay, and of the others those with the greatest sums of weights, up to n_keep keys in all.
 //
-// Bound: HBM, one read and one write of every row that moves (32 sequences of 2 K to 16 K keys down to 4096, 8 KV heads of 128,
-// 926 MB: 152 us, 6.1 TB/s; alone the selection is 24 us of that, the move 132, 7.0 TB/s); one short sequence is two
-// launches' latency (2049 keys down to 1024: 10.5 us, alone 6 and 3.4).
+// Cannot do without: one read and one write of every row that moves.  Figures here and below are of evictions with new weights each
+// time and L2 cold, in which all but the first few rows move.  32 sequences of 2 K to 16 K keys down to 4096, 8 KV heads of 128: 926 MB
+// in 237 us, 3.9 TB/s; the selection is 27 us of that, the move 203, 4.5 TB/s: before each step's rows stand two
+// latencies, the list's entry and then the table's.  One short sequence is latency (2049 keys down to 1024 17 us, the selection 9, the
+// move 8).  Evicting a cache again whose best keys lie in front already moves the recent ones alone: 157 and 15 us.
 //
 // Two launches:
 //   evict_select_kernel : one CTA or cluster of CTAs per (sequence, KV head) finds the weight T of the last key that stays by radix selection
@@ -389,9 +391,10 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_few_kernel(const Evic
   if (bad) atomicOr(p.status, kStatusOutOfRange);
 }
 
-// 128 bytes of a row per CTA, or 32 where those CTAs would not fill the SMs.  Both launches of an eviction, 8 KV heads of 128: one
-// sequence of 2049 keys to 1024 11.7 us with the former kernel in columns of 32 bytes, 10.5 with the latter, four of 4096 to
-// 2048 20.9 and 18.0; 64 of 1000 to 500 43.7 and 47.1 (with the latter in columns of 128), 32 of up to 16 K to 4096 152.3 and 154.4.
+// 128 bytes of a row per CTA, or 32 where those CTAs would be fewer than two per SM.  Both launches with the former kernel / the latter,
+// us, 8 KV heads of 128: one sequence of 2049 keys to 1024 29.7 / 17.4, of 8192 to 4096 76.8 / 33.8, of 100000 to 16384 294 / 120; sequences of
+// 4096 to 2048, four 50.0 / 35.8, nine 72.8 / 58.3, ten (the line) 74.8 / 64.5, twelve 74.7 / 74.2, sixteen 74.8 / 89.1;
+// of 1000 to 500, ten 25.6 / 27.6, sixteen 27.7 / 37.9, sixty-four 72.7 / 118; 32 of up to 16 K to 4096 238 / 276.
 int launch_move(const EvictParams& p, int batch, int head_dim, cudaStream_t st) {
   static std::atomic<bool> set[64] = {};  // per device
   int dev = 0;
