@@ -348,6 +348,11 @@ PyObject* decode_ragged(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (ws) same_device(*ws, q, "the plan's workspace");
     if (out_in) same_device(*out_in, q, "out");
     if (lse_in) same_device(*lse_in, q, "lse");
+    if (out_in && (out_in->scalar_type() != at::kBFloat16 || out_in->dim() < 3 || out_in->size(0) != r.batch || out_in->size(1) != r.heads ||
+                   out_in->size(-1) != r.d || out_in->stride(-1) != 1 || out_in->numel() != r.batch * r.heads * r.d))
+      throw ValueError("out must be bf16 [batch, n_head, head_dim]");
+    if (lse_in && (lse_in->scalar_type() != at::kFloat || !lse_in->is_contiguous() || lse_in->numel() != r.batch * r.heads))
+      throw ValueError("lse must be a contiguous float32 tensor [batch, n_head]");
     a.q = q.data_ptr();
     a.q_stride[0] = r.stride_b;
     a.q_stride[1] = r.stride_h;
